@@ -108,7 +108,9 @@ L0B_API l0b_status l0b_device_stream(l0b_device* dev, void** stream);
 L0B_API l0b_status l0b_device_graph_stats(l0b_device* dev, int64_t* built, int64_t* reused,
                                           int64_t* updated);
 /* Reads and clears the device's error flag: nonzero when a kernel's bounded wait (a pipeline barrier
- * that never completed) gave up instead of hanging; the results of that launch are invalid. */
+ * that never completed) gave up instead of hanging; the results of that launch are invalid. Bit 1 (value
+ * 2): a start, position or length that a packed or int8-cache op read on the device lay outside its
+ * buffers; the op touched nothing outside them, and the rows concerned were cut or left as they were. */
 L0B_API l0b_status l0b_device_error_status(l0b_device* dev, int32_t* code);
 /* Enables (1) or disables (0) programmatic dependent launch between consecutive kernels. */
 L0B_API l0b_status l0b_device_set_pdl(l0b_device* dev, int32_t enabled);
@@ -264,6 +266,68 @@ L0B_API l0b_status l0b_attention_execute_prefill(l0b_suite* s, l0b_device* d, l0
                                                  l0b_buffer* kc, l0b_buffer* vc, l0b_buffer* out,
                                                  int32_t head_dim, int32_t n_heads, int32_t n_kv_heads,
                                                  int32_t pos0, int32_t tokens, int32_t max_seq);
+
+/* Attention over several whole prompts in one call, causal, packed without padding (no counterpart in the
+ * reference, which prefills one sequence at a time, L/LlmDecoderLayer.cs:369-371). Sequence i of `count` has the
+ * query rows [q_starts[i], q_starts[i + 1]) of q / out and the key and value rows [kv_starts[i], kv_starts[i + 1])
+ * of k / v (i32 [count + 1] each, ascending, read on the device; kv_starts NULL: the same as q_starts). With n
+ * query and m key rows, query t stands at position m - n + t and attends to keys [0, that position]: m > n
+ * continues a prefix whose keys come first; a query with no key to see (m < n) gives zeros. out = softmax(q K^T /
+ * sqrt(hd)) V per head, query head h reading KV head h / (nH / nKv). Rows outside every sequence are left as they were.
+ *
+ * q [tokens, nH * hd] and out: f32, or the type of k and v; k, v [kv_tokens, nKv * hd]: f16 or bf16 (the types a
+ * KvCacheStore writes; stored at position 0 the rows of several prompts are such a packed buffer). Row strides
+ * in elements (<= 0: packed rows), so q, k and v may be column views of one stacked projection. k, v and 16-bit q
+ * rows start on 16 bytes (base and stride). hd 64 or 128; count <= 4096. out must not overlap the inputs.
+ * f32 queries keep about f32 accuracy (queries and probabilities enter the MMA as sums of 16-bit terms); 16-bit
+ * queries meet probabilities rounded to their own type, summed in f32. A masked key's or value's contents never
+ * reach a row, whatever they are. */
+L0B_API l0b_status l0b_attention_execute_packed(l0b_suite* s, l0b_device* d, l0b_buffer* q, l0b_buffer* k,
+                                                l0b_buffer* v, l0b_buffer* out, l0b_buffer* q_starts,
+                                                l0b_buffer* kv_starts, int32_t head_dim, int32_t n_heads,
+                                                int32_t n_kv_heads, int32_t count, int32_t tokens,
+                                                int32_t kv_tokens, int64_t q_stride, int64_t k_stride,
+                                                int64_t v_stride, int64_t out_stride);
+
+/* ---- KV cache in int8 (half the bytes of a 16-bit cache; no counterpart in the reference, whose cache is f32,
+ * L/LlmKvCache.cs) ----
+ * Kc, Vc: i8 [count, max_seq, nKv * hd]. k_scales, v_scales: f32 [count, ceil(max_seq / block), nKv], one scale per
+ * block of `block` slots (32, 64 or 128) and KV head, K and V apart: a slot holds code * scale. Sequence i of a
+ * call is row i of these buffers (l0b_buffer_view names a run of rows). All zero (as allocated) is a valid empty
+ * cache. starts: i32 [count + 1], the packed rows of each sequence as in l0b_attention_execute_packed; NULL: one
+ * row a sequence (tokens == count). positions / lengths: i32 [count]. All are read on the device, so a recorded
+ * command list follows their contents. hd 64 or 128; count <= 4096.
+ *
+ * Store: rows of k / v [tokens, nKv * hd] (f32, f16 or bf16, row strides as above) go to slots positions[i],
+ * positions[i] + 1, ... The scale of a block is f32(max|x| / 127) over its new rows and the codes are
+ * rint(x / scale), ties to even, exactly (no rounding of the quotient first). Where a block keeps slots below the
+ * first new one, its scale never falls below what it was, and when it grows the kept codes c become
+ * rint(c * old / new). The slots of the block behind the last new row no longer hold anything (a store cuts the
+ * sequence there). A scale of 0 or one that is not finite has codes 0: a block that received an infinity or a NaN
+ * reads back as NaN until it is stored anew from its first slot. Storing the same rows again changes nothing. */
+L0B_API l0b_status l0b_kv_cache_q8_store(l0b_suite* s, l0b_device* d, l0b_buffer* k, l0b_buffer* v, l0b_buffer* kc,
+                                         l0b_buffer* vc, l0b_buffer* k_scales, l0b_buffer* v_scales,
+                                         l0b_buffer* starts, l0b_buffer* positions, int32_t n_kv_heads,
+                                         int32_t head_dim, int32_t block, int32_t max_seq, int32_t count,
+                                         int32_t tokens, int64_t k_stride, int64_t v_stride);
+/* Load: slots positions[i], positions[i] + 1, ... of sequence i as rows of k / v (f32, f16 or bf16): a cached
+ * prefix for l0b_attention_execute_packed, or a sequence to keep elsewhere. */
+L0B_API l0b_status l0b_kv_cache_q8_load(l0b_suite* s, l0b_device* d, l0b_buffer* kc, l0b_buffer* vc,
+                                        l0b_buffer* k_scales, l0b_buffer* v_scales, l0b_buffer* k, l0b_buffer* v,
+                                        l0b_buffer* starts, l0b_buffer* positions, int32_t n_kv_heads,
+                                        int32_t head_dim, int32_t block, int32_t max_seq, int32_t count,
+                                        int32_t tokens, int64_t k_stride, int64_t v_stride);
+/* Attention.Execute over the int8 cache for `count` sequences at once: sequence i holds lengths[i] slots, the last
+ * of them the positions of its n query rows (one, or a few drafted tokens), and query t attends to slots
+ * [0, lengths[i] - n + t] (none: zeros). q [tokens, nH * hd] and out: f32, f16 or bf16, one type; row strides in
+ * elements (<= 0: packed rows). Products and sums keep about f32 accuracy against the cache's values. One launch
+ * for any mix of lengths. Long blocks of queries are better served by Load and l0b_attention_execute_packed. */
+L0B_API l0b_status l0b_attention_execute_q8(l0b_suite* s, l0b_device* d, l0b_buffer* q, l0b_buffer* kc,
+                                            l0b_buffer* vc, l0b_buffer* k_scales, l0b_buffer* v_scales,
+                                            l0b_buffer* out, l0b_buffer* starts, l0b_buffer* lengths,
+                                            int32_t head_dim, int32_t n_heads, int32_t n_kv_heads, int32_t block,
+                                            int32_t max_seq, int32_t count, int32_t tokens, int64_t q_stride,
+                                            int64_t out_stride);
 
 /* Decode attention (the l0b_attention_execute computation, one query token over cache slots
  * [0, seq_len)) that allocates nothing, for callers that cannot allocate device memory during a call:

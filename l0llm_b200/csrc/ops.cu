@@ -421,6 +421,228 @@ L0B_API l0b_status l0b_attention_execute_prefill(l0b_suite* s, l0b_device* d, l0
     return attention_common(s, d, q, kc, vc, out, head_dim, n_heads, n_kv_heads, pos0, 1, tokens, max_seq, true);
 }
 
+// A buffer of `rows` rows of `width` elements, `stride` elements apart, on device d.
+static l0b_status need_rows(l0b_device* d, l0b_buffer* b, const char* name, long long rows, long long width,
+                            int64_t* stride) {
+    L0B_REQUIRE(b, L0B_ERR_ARGUMENT, "%s is null", name);
+    L0B_REQUIRE(b->dev->index == d->index, L0B_ERR_ARGUMENT, "%s belongs to another device", name);
+    if (*stride <= 0) *stride = width;
+    L0B_REQUIRE(*stride >= width, L0B_ERR_ARGUMENT, "%s row stride %lld is below the row width %lld", name,
+                (long long)*stride, width);
+    L0B_REQUIRE(rows <= 1 || *stride <= (INT64_MAX - width) / (rows - 1), L0B_ERR_OUT_OF_RANGE,
+                "%s row stride %lld is too large", name, (long long)*stride);
+    const long long want = rows > 0 ? (rows - 1) * static_cast<long long>(*stride) + width : 0;
+    L0B_REQUIRE(b->count >= want, L0B_ERR_ARGUMENT, "%s holds %lld elements, need %lld", name, (long long)b->count, want);
+    return L0B_OK;
+}
+
+static l0b_status need_on(l0b_device* d, l0b_buffer* b, const char* name, l0b_dtype t, long long count) {
+    L0B_TRY(need(b, name, t, count));
+    L0B_REQUIRE(b->dev->index == d->index, L0B_ERR_ARGUMENT, "%s belongs to another device", name);
+    return L0B_OK;
+}
+
+static l0b_status need_16_bytes(l0b_buffer* b, const char* name, int64_t stride) {
+    L0B_REQUIRE(reinterpret_cast<uintptr_t>(b->ptr) % 16 == 0 && stride * dtype_size(b->dtype) % 16 == 0,
+                L0B_ERR_ARGUMENT, "%s rows must start on 16 bytes (row stride %lld elements)", name, (long long)stride);
+    return L0B_OK;
+}
+
+static l0b_status check_seq_shape(int hd, int nh, int nkv, int count, int tokens) {
+    L0B_REQUIRE(nh > 0 && nkv > 0 && nh % nkv == 0, L0B_ERR_ARGUMENT, "heads %d are not a multiple of KV heads %d", nh, nkv);
+    L0B_REQUIRE(hd == 64 || hd == 128, L0B_ERR_UNSUPPORTED, "attention head_dim %d is not supported (64, 128)", hd);
+    L0B_REQUIRE(count >= 0 && count <= kMaxSequences, L0B_ERR_OUT_OF_RANGE, "count %d outside [0, %d]", count, kMaxSequences);
+    L0B_REQUIRE(tokens >= 0, L0B_ERR_OUT_OF_RANGE, "tokens %d is negative", tokens);
+    L0B_REQUIRE(static_cast<long long>(nh) * hd <= INT32_MAX, L0B_ERR_OUT_OF_RANGE, "heads %d", nh);
+    return L0B_OK;
+}
+
+L0B_API l0b_status l0b_attention_execute_packed(l0b_suite* s, l0b_device* d, l0b_buffer* q, l0b_buffer* k,
+                                                l0b_buffer* v, l0b_buffer* out, l0b_buffer* q_starts,
+                                                l0b_buffer* kv_starts, int32_t head_dim, int32_t n_heads,
+                                                int32_t n_kv_heads, int32_t count, int32_t tokens, int32_t kv_tokens,
+                                                int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                                int64_t out_stride) {
+    L0B_TRY(check_suite(s, d));
+    L0B_TRY(check_seq_shape(head_dim, n_heads, n_kv_heads, count, tokens));
+    L0B_REQUIRE(kv_tokens >= 0, L0B_ERR_OUT_OF_RANGE, "kvTokens %d is negative", kv_tokens);
+    const long long qd = static_cast<long long>(n_heads) * head_dim, kvd = static_cast<long long>(n_kv_heads) * head_dim;
+    L0B_TRY(need_rows(d, q, "q", tokens, qd, &q_stride));
+    L0B_TRY(need_rows(d, k, "k", kv_tokens, kvd, &k_stride));
+    L0B_TRY(need_rows(d, v, "v", kv_tokens, kvd, &v_stride));
+    L0B_TRY(need_rows(d, out, "out", tokens, qd, &out_stride));
+    L0B_REQUIRE(k->dtype == L0B_F16 || k->dtype == L0B_BF16, L0B_ERR_ARGUMENT, "k must be an f16 or bf16 buffer, got %s",
+                dtype_name(k->dtype));
+    L0B_REQUIRE(v->dtype == k->dtype, L0B_ERR_ARGUMENT, "k and v differ in dtype");
+    L0B_REQUIRE(q->dtype == L0B_F32 || q->dtype == k->dtype, L0B_ERR_ARGUMENT, "q must be f32 or the type of k (%s), got %s",
+                dtype_name(k->dtype), dtype_name(q->dtype));
+    L0B_REQUIRE(out->dtype == q->dtype, L0B_ERR_ARGUMENT, "out must have the type of q (%s), got %s",
+                dtype_name(q->dtype), dtype_name(out->dtype));
+    L0B_TRY(need_16_bytes(k, "k", k_stride));
+    L0B_TRY(need_16_bytes(v, "v", v_stride));
+    L0B_TRY(need_16_bytes(q, "q", q_stride));
+    L0B_TRY(need_16_bytes(out, "out", out_stride));
+    L0B_TRY(need_on(d, q_starts, "qStarts", L0B_I32, static_cast<long long>(count) + 1));
+    if (kv_starts) {
+        L0B_TRY(need_on(d, kv_starts, "kvStarts", L0B_I32, static_cast<long long>(count) + 1));
+    } else {
+        L0B_REQUIRE(kv_tokens == tokens, L0B_ERR_ARGUMENT, "without kvStarts kvTokens (%d) must equal tokens (%d)",
+                    kv_tokens, tokens);
+    }
+    if (count == 0 || tokens == 0) return L0B_OK;
+    L0B_CHECK_CUDA(cudaSetDevice(d->index));
+    PackedAttnParams p = {};
+    p.q = q->ptr;
+    p.k = k->ptr;
+    p.v = v->ptr;
+    p.out = out->ptr;
+    p.q_starts = static_cast<const int*>(q_starts->ptr);
+    p.kv_starts = kv_starts ? static_cast<const int*>(kv_starts->ptr) : p.q_starts;
+    p.q_dtype = q->dtype;
+    p.kv_dtype = k->dtype;
+    p.hd = head_dim;
+    p.nh = n_heads;
+    p.nkv = n_kv_heads;
+    p.count = count;
+    p.tokens = tokens;
+    p.kv_tokens = kv_tokens;
+    p.q_stride = q_stride;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.out_stride = out_stride;
+    p.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(head_dim)));
+    p.error = d->error_flag;
+    return k_attention_packed(s, d, p);
+}
+
+// The int8 cache's own buffers: codes [count, max_seq, kv_dim] and scales [count, blocks, n_kv_heads].
+static l0b_status check_q8_cache(l0b_device* d, l0b_buffer* kc, l0b_buffer* vc, l0b_buffer* ks, l0b_buffer* vs,
+                                 l0b_buffer* starts, int nkv, int hd, int block, int max_seq, int count, int tokens) {
+    L0B_REQUIRE(block == 32 || block == 64 || block == 128, L0B_ERR_UNSUPPORTED, "block %d is not supported (32, 64, 128)",
+                block);
+    L0B_REQUIRE(max_seq > 0, L0B_ERR_OUT_OF_RANGE, "maxSeq %d must be positive", max_seq);
+    const long long blocks = (static_cast<long long>(max_seq) + block - 1) / block;
+    const long long slots = static_cast<long long>(count) * max_seq;  // < 2^43
+    L0B_REQUIRE(slots <= INT32_MAX, L0B_ERR_OUT_OF_RANGE, "count %d * maxSeq %d slots exceed %d", count, max_seq, INT32_MAX);
+    const long long codes = slots * nkv * hd, scales = count * blocks * nkv;
+    L0B_TRY(need_on(d, kc, "Kc", L0B_I8, codes));
+    L0B_TRY(need_on(d, vc, "Vc", L0B_I8, codes));
+    L0B_TRY(need_on(d, ks, "kScales", L0B_F32, scales));
+    L0B_TRY(need_on(d, vs, "vScales", L0B_F32, scales));
+    L0B_TRY(need_16_bytes(kc, "Kc", static_cast<int64_t>(nkv) * hd));
+    L0B_TRY(need_16_bytes(vc, "Vc", static_cast<int64_t>(nkv) * hd));
+    if (starts) {
+        L0B_TRY(need_on(d, starts, "starts", L0B_I32, static_cast<long long>(count) + 1));
+    } else {
+        L0B_REQUIRE(tokens == count, L0B_ERR_ARGUMENT, "without starts there is one row a sequence: tokens %d, count %d",
+                    tokens, count);
+    }
+    return L0B_OK;
+}
+
+static l0b_status kv_q8_common(l0b_suite* s, l0b_device* d, l0b_buffer* k, l0b_buffer* v, l0b_buffer* kc, l0b_buffer* vc,
+                               l0b_buffer* ks, l0b_buffer* vs, l0b_buffer* starts, l0b_buffer* positions, int nkv, int hd,
+                               int block, int max_seq, int count, int tokens, int64_t k_stride, int64_t v_stride,
+                               KvQ8Params* p) {
+    L0B_TRY(check_suite(s, d));
+    L0B_TRY(check_seq_shape(hd, nkv, nkv, count, tokens));
+    L0B_TRY(check_q8_cache(d, kc, vc, ks, vs, starts, nkv, hd, block, max_seq, count, tokens));
+    L0B_TRY(need_rows(d, k, "k", tokens, static_cast<long long>(nkv) * hd, &k_stride));
+    L0B_TRY(need_rows(d, v, "v", tokens, static_cast<long long>(nkv) * hd, &v_stride));
+    L0B_TRY(need_float(k, "k", 0));
+    L0B_REQUIRE(v->dtype == k->dtype, L0B_ERR_ARGUMENT, "k and v differ in dtype");
+    L0B_TRY(need_16_bytes(k, "k", k_stride));
+    L0B_TRY(need_16_bytes(v, "v", v_stride));
+    L0B_TRY(need_on(d, positions, "positions", L0B_I32, count));
+    L0B_CHECK_CUDA(cudaSetDevice(d->index));
+    p->k = k->ptr;
+    p->v = v->ptr;
+    p->kc = static_cast<int8_t*>(kc->ptr);
+    p->vc = static_cast<int8_t*>(vc->ptr);
+    p->ks = F(ks);
+    p->vs = F(vs);
+    p->starts = starts ? static_cast<const int*>(starts->ptr) : nullptr;
+    p->positions = static_cast<const int*>(positions->ptr);
+    p->dtype = k->dtype;
+    p->nkv = nkv;
+    p->hd = hd;
+    p->block = block;
+    p->max_seq = max_seq;
+    p->blocks = (max_seq + block - 1) / block;
+    p->count = count;
+    p->tokens = tokens;
+    p->k_stride = k_stride;
+    p->v_stride = v_stride;
+    p->error = d->error_flag;
+    return L0B_OK;
+}
+
+L0B_API l0b_status l0b_kv_cache_q8_store(l0b_suite* s, l0b_device* d, l0b_buffer* k, l0b_buffer* v, l0b_buffer* kc,
+                                         l0b_buffer* vc, l0b_buffer* k_scales, l0b_buffer* v_scales, l0b_buffer* starts,
+                                         l0b_buffer* positions, int32_t n_kv_heads, int32_t head_dim, int32_t block,
+                                         int32_t max_seq, int32_t count, int32_t tokens, int64_t k_stride,
+                                         int64_t v_stride) {
+    KvQ8Params p = {};
+    L0B_TRY(kv_q8_common(s, d, k, v, kc, vc, k_scales, v_scales, starts, positions, n_kv_heads, head_dim, block, max_seq,
+                         count, tokens, k_stride, v_stride, &p));
+    return count == 0 || tokens == 0 ? L0B_OK : k_kv_q8_store(d, p);
+}
+
+L0B_API l0b_status l0b_kv_cache_q8_load(l0b_suite* s, l0b_device* d, l0b_buffer* kc, l0b_buffer* vc,
+                                        l0b_buffer* k_scales, l0b_buffer* v_scales, l0b_buffer* k, l0b_buffer* v,
+                                        l0b_buffer* starts, l0b_buffer* positions, int32_t n_kv_heads, int32_t head_dim,
+                                        int32_t block, int32_t max_seq, int32_t count, int32_t tokens, int64_t k_stride,
+                                        int64_t v_stride) {
+    KvQ8Params p = {};
+    L0B_TRY(kv_q8_common(s, d, k, v, kc, vc, k_scales, v_scales, starts, positions, n_kv_heads, head_dim, block, max_seq,
+                         count, tokens, k_stride, v_stride, &p));
+    return count == 0 || tokens == 0 ? L0B_OK : k_kv_q8_load(d, p);
+}
+
+L0B_API l0b_status l0b_attention_execute_q8(l0b_suite* s, l0b_device* d, l0b_buffer* q, l0b_buffer* kc, l0b_buffer* vc,
+                                            l0b_buffer* k_scales, l0b_buffer* v_scales, l0b_buffer* out,
+                                            l0b_buffer* starts, l0b_buffer* lengths, int32_t head_dim, int32_t n_heads,
+                                            int32_t n_kv_heads, int32_t block, int32_t max_seq, int32_t count,
+                                            int32_t tokens, int64_t q_stride, int64_t out_stride) {
+    L0B_TRY(check_suite(s, d));
+    L0B_TRY(check_seq_shape(head_dim, n_heads, n_kv_heads, count, tokens));
+    L0B_TRY(check_q8_cache(d, kc, vc, k_scales, v_scales, starts, n_kv_heads, head_dim, block, max_seq, count, tokens));
+    const long long qd = static_cast<long long>(n_heads) * head_dim;
+    L0B_TRY(need_rows(d, q, "q", tokens, qd, &q_stride));
+    L0B_TRY(need_rows(d, out, "out", tokens, qd, &out_stride));
+    L0B_TRY(need_float(q, "q", 0));
+    L0B_REQUIRE(out->dtype == q->dtype, L0B_ERR_ARGUMENT, "out must have the type of q (%s), got %s",
+                dtype_name(q->dtype), dtype_name(out->dtype));
+    L0B_TRY(need_16_bytes(q, "q", q_stride));
+    L0B_TRY(need_16_bytes(out, "out", out_stride));
+    L0B_TRY(need_on(d, lengths, "lengths", L0B_I32, count));
+    if (count == 0 || tokens == 0) return L0B_OK;
+    L0B_CHECK_CUDA(cudaSetDevice(d->index));
+    AttnQ8Params p = {};
+    p.q = q->ptr;
+    p.out = out->ptr;
+    p.kc = static_cast<const int8_t*>(kc->ptr);
+    p.vc = static_cast<const int8_t*>(vc->ptr);
+    p.ks = F(k_scales);
+    p.vs = F(v_scales);
+    p.starts = starts ? static_cast<const int*>(starts->ptr) : nullptr;
+    p.lengths = static_cast<const int*>(lengths->ptr);
+    p.dtype = q->dtype;
+    p.hd = head_dim;
+    p.nh = n_heads;
+    p.nkv = n_kv_heads;
+    p.block = block;
+    p.max_seq = max_seq;
+    p.blocks = (max_seq + block - 1) / block;
+    p.count = count;
+    p.tokens = tokens;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(head_dim)));
+    p.error = d->error_flag;
+    return k_attention_q8(s, d, p);
+}
+
 L0B_API l0b_status l0b_sigmoid_gate_execute(l0b_suite* s, l0b_device* d, l0b_buffer* x, l0b_buffer* gate, int32_t n) {
     L0B_TRY(check_suite(s, d));
     L0B_REQUIRE(n >= 0, L0B_ERR_OUT_OF_RANGE, "n %d", n);

@@ -81,6 +81,61 @@ size_t attention_part_floats(int batch, int nh, int max_splits, int hd);
 // Picks the split length for a cache of max_seq positions and `work_items` (batch * nKv) rows.
 void attention_pick_split(int max_seq, int work_items, int sm_count, int* chunk, int* max_splits);
 
+// ------------------------------------------------------------------------------------------------
+// Packed prompts (attention_packed.cu) and the int8 KV cache (kv_q8.cu, attention_q8.cu)
+// ------------------------------------------------------------------------------------------------
+
+constexpr int kMaxSequences = 4096;  // sequences of one packed or int8-cache call
+
+struct PackedAttnParams {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    const int* q_starts;   // [count + 1]
+    const int* kv_starts;  // [count + 1]
+    int q_dtype, kv_dtype; // q and out share q_dtype
+    int hd, nh, nkv, count, tokens, kv_tokens;
+    long long q_stride, k_stride, v_stride, out_stride;  // elements
+    float scale;           // head_dim^-0.5
+    int* error;            // device error flag: bit 1 for starts outside the buffers
+};
+l0b_status k_attention_packed(l0b_suite* s, l0b_device* d, const PackedAttnParams& p);
+
+struct KvQ8Params {
+    const void* k;         // store: rows in; load: rows out (K and V)
+    const void* v;
+    int8_t* kc;
+    int8_t* vc;
+    float* ks;
+    float* vs;
+    const int* starts;     // [count + 1], or null: one row a sequence
+    const int* positions;  // [count]
+    int dtype;             // of the rows
+    int nkv, hd, block, max_seq, blocks, count, tokens;  // blocks: scale rows per sequence
+    long long k_stride, v_stride;  // elements
+    int* error;
+};
+l0b_status k_kv_q8_store(l0b_device* d, const KvQ8Params& p);
+l0b_status k_kv_q8_load(l0b_device* d, const KvQ8Params& p);
+
+struct AttnQ8Params {
+    const void* q;
+    void* out;
+    const int8_t* kc;
+    const int8_t* vc;
+    const float* ks;
+    const float* vs;
+    const int* starts;   // [count + 1], or null: one row a sequence
+    const int* lengths;  // [count]
+    int dtype;           // of q and out
+    int hd, nh, nkv, block, max_seq, blocks, count, tokens;
+    long long q_stride, out_stride;  // elements
+    float scale;
+    int* error;
+};
+l0b_status k_attention_q8(l0b_suite* s, l0b_device* d, const AttnQ8Params& p);
+
 // Device sampling (LlmSampler.Sample): validates the parameters (top_k within the select's 1024
 // candidates when T > 0).
 l0b_status sample_check(float temperature, float top_p, int top_k, float penalty, int vocab);

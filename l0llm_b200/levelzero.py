@@ -161,6 +161,10 @@ def load_library() -> C.CDLL:
         "l0b_kv_cache_store_execute_rows": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32]),
         "l0b_attention_execute": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32]),
         "l0b_attention_execute_prefill": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32]),
+        "l0b_attention_execute_packed": (i32, [vp] * 8 + [i32] * 6 + [i64] * 4),
+        "l0b_attention_execute_q8": (i32, [vp] * 10 + [i32] * 7 + [i64] * 2),
+        "l0b_kv_cache_q8_store": (i32, [vp] * 10 + [i32] * 6 + [i64] * 2),
+        "l0b_kv_cache_q8_load": (i32, [vp] * 10 + [i32] * 6 + [i64] * 2),
         "l0b_sigmoid_gate_execute": (i32, [vp, vp, vp, vp, i32]),
         "l0b_swiglu_execute": (i32, [vp, vp, vp, vp, i32]),
         "l0b_add_execute": (i32, [vp, vp, vp, vp, i32]),
@@ -492,6 +496,37 @@ class _Attention(_Op):
                                                    hd, nH, nKv, pos0, tokens, maxSeq))
 
 
+    def ExecutePacked(self, dev, q, k, v, out, qStarts, kvStarts, hd, nH, nKv, count, tokens, kvTokens, qStride=0,
+                      kStride=0, vStride=0, outStride=0):
+        """Causal attention over `count` packed sequences (kvStarts None: the same rows as qStarts)."""
+        check(self.L.l0b_attention_execute_packed(self._s(), dev.handle, q.handle, k.handle, v.handle, out.handle,
+                                                  qStarts.handle, _h(kvStarts), hd, nH, nKv, count, tokens, kvTokens,
+                                                  qStride, kStride, vStride, outStride))
+
+    def ExecuteQ8(self, dev, q, Kc, Vc, kScales, vScales, out, starts, lengths, hd, nH, nKv, block, maxSeq, count,
+                  tokens, qStride=0, outStride=0):
+        """Attention of `count` sequences over the int8 cache (starts None: one query row each)."""
+        check(self.L.l0b_attention_execute_q8(self._s(), dev.handle, q.handle, Kc.handle, Vc.handle, kScales.handle,
+                                              vScales.handle, out.handle, _h(starts), lengths.handle, hd, nH, nKv,
+                                              block, maxSeq, count, tokens, qStride, outStride))
+
+
+class _KvCacheQ8(_Op):
+    """The int8 KV cache: codes [count, maxSeq, nKv * hd] and one f32 scale per (block of slots, KV head)."""
+
+    def Store(self, dev, k, v, Kc, Vc, kScales, vScales, starts, positions, nKv, hd, block, maxSeq, count, tokens,
+              kStride=0, vStride=0):
+        check(self.L.l0b_kv_cache_q8_store(self._s(), dev.handle, k.handle, v.handle, Kc.handle, Vc.handle,
+                                           kScales.handle, vScales.handle, _h(starts), positions.handle, nKv, hd,
+                                           block, maxSeq, count, tokens, kStride, vStride))
+
+    def Load(self, dev, Kc, Vc, kScales, vScales, k, v, starts, positions, nKv, hd, block, maxSeq, count, tokens,
+             kStride=0, vStride=0):
+        check(self.L.l0b_kv_cache_q8_load(self._s(), dev.handle, Kc.handle, Vc.handle, kScales.handle, vScales.handle,
+                                          k.handle, v.handle, _h(starts), positions.handle, nKv, hd, block, maxSeq,
+                                          count, tokens, kStride, vStride))
+
+
 class _Unary(_Op):
     def __init__(self, suite, fn):
         super().__init__(suite)
@@ -574,6 +609,7 @@ class LlmKernelSuite:
         self.RoPE = _RoPE(self)
         self.KvCacheStore = _KvCacheStore(self)
         self.Attention = _Attention(self)
+        self.KvCacheQ8 = _KvCacheQ8(self)
         self.SigmoidGate = _Unary(self, "l0b_sigmoid_gate_execute")
         self.SwiGLU = _Unary(self, "l0b_swiglu_execute")
         self.Add = _Unary(self, "l0b_add_execute")
