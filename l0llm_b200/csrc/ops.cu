@@ -44,6 +44,8 @@ l0b_suite::~l0b_suite() {
     if (gdn_rec) cudaFree(gdn_rec);
     if (split_counters) cudaFree(split_counters);
     if (ks_acc) cudaFree(ks_acc);
+    if (q8_part) cudaFree(q8_part);
+    if (q8_counters) cudaFree(q8_counters);
 }
 
 namespace {
@@ -102,6 +104,10 @@ L0B_API l0b_status l0b_suite_create(l0b_device* dev, l0b_suite** out) {
     L0B_CHECK_CUDA(cudaMemsetAsync(s->split_counters, 0, sizeof(unsigned) * kSuiteSplitTiles, dev->stream));
     L0B_CHECK_CUDA(cudaMalloc(&s->ks_acc, sizeof(long long) * kSuiteKsRows));
     L0B_CHECK_CUDA(cudaMemsetAsync(s->ks_acc, 0, sizeof(long long) * kSuiteKsRows, dev->stream));
+    const size_t teams = static_cast<size_t>(kQ8TeamsPerSm) * dev->sm_count;
+    L0B_CHECK_CUDA(cudaMalloc(&s->q8_part, sizeof(float) * 2 * teams * 16 * (128 + 2)));
+    L0B_CHECK_CUDA(cudaMalloc(&s->q8_counters, sizeof(unsigned) * teams));
+    L0B_CHECK_CUDA(cudaMemsetAsync(s->q8_counters, 0, sizeof(unsigned) * teams, dev->stream));
     L0B_CHECK_CUDA(cudaStreamSynchronize(dev->stream));
     *out = s.release();
     return L0B_OK;

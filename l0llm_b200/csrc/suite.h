@@ -15,6 +15,8 @@ constexpr int kPrefillRows = 512;
 constexpr int kSuiteSplitTiles = 4096;
 // Output rows the suite's k-split GEMV row sums cover (l0b_linear_fused over blocked int8 weights).
 constexpr int kSuiteKsRows = 16 * kSuiteSplitTiles;
+// Teams of warps of the int8-cache attention per SM, at most: parts of shared items it may leave per launch.
+constexpr int kQ8TeamsPerSm = 3;
 }  // namespace l0b
 
 struct l0b_suite {
@@ -33,6 +35,10 @@ struct l0b_suite {
     // Exact int64 row sums of the k-split GEMV [kSuiteKsRows], zero at rest (every launch leaves them
     // zero); its tile-group counters are split_counters.
     long long* ks_acc = nullptr;
+    // Int8-cache attention: two parts per team (16 columns of 128 dims, then 16 (maximum, sum) pairs) and an
+    // arrival counter per team, zero at rest. Launches of one stream take turns, so all share them.
+    float* q8_part = nullptr;
+    unsigned* q8_counters = nullptr;
     std::map<std::pair<int, double>, float*> rope_tables;
     ~l0b_suite();
 };
