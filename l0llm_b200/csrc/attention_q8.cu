@@ -7,12 +7,15 @@
 // fetched by its own TMA two tiles ahead, segments ahead included, so HBM stays busy through their ends.
 //
 // The query columns of an item are the rows that share its keys (the heads of a group, times the tokens): the MMA's
-// n = 8 (NT tiles of it). Keys are its m: S^T[16 slots, 8 columns] = K Q^T with the int8 keys turned to f16 in
-// registers, exactly (byte b ^ 0x80 under the exponent of 1024, minus 1152), and each query column scaled by a power
-// of two and split in hi + lo f16 terms. O^T[16 dims, 8] += V^T P^T likewise, P^T in hi + lo terms made from the
-// scores' own registers by movmatrix. So no product is padded to 16 query rows and nothing but the raw codes crosses
-// shared memory. A block's key scale multiplies the scores; its value scale the product of its 32 slots, summed in
-// f32 outside the MMA, which truncates its sums: 32 slots a sum keep that below the f32 rounding of the rest.
+// n = 8 (NT tiles of it). Keys are its m: S^T[16 slots, 8 columns] = K Q^T on the integer MMA, the codes as they lie
+// in the cache and each query column as three base-256 digits of its values, scaled by a power of two to 23 bits of
+// the column's largest: exact sums and no conversion (turning keys to f16 took 160 of 790 instructions a tile).
+// O^T[16 dims, 8] += V^T P^T takes the codes as f16, exactly (byte b ^ 0x80 under the exponent of 1024, minus 1152),
+// and P^T in hi + lo f16 terms made from the scores' own registers by movmatrix; digits there would cost more than
+// they save, since every output would have to be converted for every tile. No product is padded to 16 query rows,
+// and nothing but the raw codes crosses shared memory. A block's key scale multiplies the scores; its value scale
+// the product of its 32 slots, summed in f32 outside the MMA, which truncates its sums: 32 slots a sum keep that
+// below the f32 rounding of the rest.
 // Softmax online, per warp and column, in exp2; weights carry a factor 2^14 that keeps their lo terms normal f16.
 //
 // At a segment's end the team's warps meet in shared memory (each in the ring stage it has just read). An item that
@@ -47,12 +50,12 @@ struct Q8Launch {
 
 // What a warp needs to know of one item, and the walk over items.
 struct Item {
-    int seq;        // sequence
-    int sub, subs;  // KV head * column groups + column group; their number
-    int cgroups;    // column groups of the sequence
+    int seq;            // sequence
+    int head, cg;       // KV head, column group
+    int cgroups;        // column groups of the sequence
     int tiles;
-    int len, n, row0;  // slots held, query rows, first packed row
-    long long base;    // first unit
+    int len, n, row0;   // slots held, query rows, first packed row
+    long long base;     // first unit
 };
 
 template <int NT>
@@ -72,7 +75,6 @@ struct Walk {
     __device__ __forceinline__ void load_sequence(Item& it) const {
         sequence(it.seq, it.row0, it.n, it.len);
         it.cgroups = column_groups(it.n);
-        it.subs = it.cgroups * a.nkv;
         it.tiles = tiles_of(it.len);
     }
     // The item that holds unit u.
@@ -86,14 +88,18 @@ struct Walk {
         Item it;
         it.seq = lo;
         load_sequence(it);
-        it.sub = static_cast<int>((u - pre[lo]) / it.tiles);
-        it.base = pre[lo] + static_cast<long long>(it.sub) * it.tiles;
+        const int sub = static_cast<int>((u - pre[lo]) / it.tiles);
+        it.head = sub / it.cgroups;
+        it.cg = sub - it.head * it.cgroups;
+        it.base = pre[lo] + static_cast<long long>(sub) * it.tiles;
         return it;
     }
     __device__ __forceinline__ void next(Item& it) const {
         it.base += it.tiles;
-        if (++it.sub < it.subs) return;
-        it.sub = 0;
+        if (++it.cg < it.cgroups) return;
+        it.cg = 0;
+        if (++it.head < a.nkv) return;
+        it.head = 0;
         do ++it.seq;
         while (it.seq + 1 < a.count && pre[it.seq] == pre[it.seq + 1]);
         if (it.seq < a.count) load_sequence(it);
@@ -106,6 +112,20 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Byte k of each of four words, side by side.
+__device__ __forceinline__ uint32_t byte_of(const int (&x)[4], int k) {
+    const uint32_t lo = __byte_perm(x[0], x[1], k | ((4 + k) << 4)), hi = __byte_perm(x[2], x[3], k | ((4 + k) << 4));
+    return __byte_perm(lo, hi, 0x5410);
 }
 
 // Bytes (0, 1) and (2, 3) of u (codes ^ 0x80) as f16 pairs, exactly.
@@ -138,7 +158,7 @@ template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __grid_constant__ Q8Launch L) {
     constexpr int W = warps_of(NT), COLS = 8 * NT;
     constexpr int SLOTS = kTileBytes / HD, MT = SLOTS / 16, HALVES = SLOTS / 32;
-    constexpr int KS = HD / 16;   // 16-deep steps of K Q^T
+    constexpr int KS = HD / 32;   // 32-deep steps of K Q^T
     constexpr int DT_ = HD / 16;  // 16-dim tiles of O
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -229,21 +249,22 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
         return true;
     };
     float ks_q[2][HALVES], vs_q[2][HALVES];  // [0]: the next tile to read, [1]: the one behind it
+    const int block_log = 31 - __clz(a.block);
     int issued = 0;
     bool more = settle();
     auto fetch = [&](float (&ks)[HALVES], float (&vs)[HALVES]) {
-        const int st = issued & 1, kvh = fi.sub / fi.cgroups;
+        const int st = issued & 1;
         if (lane == 0) {
             const uint32_t bar = bar_addr + 8 * st, dst = ring_addr + st * 2 * kTileBytes;
             bar_expect(bar, 2 * kTileBytes);
-            const int x = kvh * HD, y = fi.seq * a.max_seq + fj * SLOTS;
+            const int x = fi.head * HD, y = fi.seq * a.max_seq + fj * SLOTS;
             tma_load(dst, &L.kmap, bar, x, y);
             tma_load(dst + kTileBytes, &L.vmap, bar, x, y);
         }
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
             const int slot = fj * SLOTS + h * 32;
-            const long long at = (static_cast<long long>(fi.seq) * a.blocks + slot / a.block) * a.nkv + kvh;
+            const long long at = (static_cast<long long>(fi.seq) * a.blocks + (slot >> block_log)) * a.nkv + fi.head;
             const bool holds = slot < fi.len;  // a block behind the sequence has no scale to speak of
             ks[h] = holds ? __ldg(a.ks + at) : 0.f;
             vs[h] = holds ? __ldg(a.vs + at) : 0.f;
@@ -263,18 +284,18 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     while (true) {
         const int j0 = static_cast<int>(u - it.base);
         const int j1 = static_cast<int>(min(static_cast<long long>(it.tiles), u1 - it.base));
-        const int kvh = it.sub / it.cgroups, c0 = (it.sub - kvh * it.cgroups) * COLS;  // first column
+        const int kvh = it.head, c0 = it.cg * COLS;  // first column
         const int cols = min(COLS, it.n * G - c0);
 
-        // Query columns: lane (g, t) holds column nt * 8 + g, the dims that its key words will hold.
-        uint32_t qh[NT][KS][2], ql[NT][KS][2];
+        // Query columns: lane (g, t) holds column nt * 8 + g, the dims that its key words will hold, as digits.
+        uint32_t qd[NT][KS][3][2];
         float factor[NT][2];  // score factor of this lane's accumulator columns nt * 8 + 2 t, + 1
         int seen[NT][2];      // slots those columns see
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int col = nt * 8 + g;
+            const int col = min(nt * 8 + g, cols - 1);
             float x[HD / 4];
-            const int tok = (c0 + min(col, cols - 1)) / G, head = (c0 + min(col, cols - 1)) - tok * G;
+            const int tok = (c0 + col) / G, head = c0 + col - tok * G;
             const T* q = static_cast<const T*>(a.q) + (it.row0 + tok) * a.q_stride + (kvh * G + head) * HD + t * 16;
 #pragma unroll
             for (int e = 0; e < HD / 4; e += 8) {
@@ -284,17 +305,34 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                 for (int i = 0; i < 8; ++i) x[e + i] = y[i];
             }
             float top = 0.f;
+            bool odd = false;  // an infinity or a NaN in the column: its scores become NaN
 #pragma unroll
-            for (int e = 0; e < HD / 4; ++e) top = fmaxf(top, fabsf(x[e]));
+            for (int e = 0; e < HD / 4; ++e) {
+                top = fmaxf(top, fabsf(x[e]));
+                odd |= !(fabsf(x[e]) < __int_as_float(0x7F800000));
+            }
+            if (odd) top = __int_as_float(0x7F800000);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^bits lifts the column's largest value to [2^13, 2^14): hi + lo keep 22 bits of it.
-            const int bits = top > 0.f && top < __int_as_float(0x7F800000) ? min(13 - ilogbf(top), 126) : 0;
-            const float up = ldexpf(1.f, bits), f = ldexpf(a.scale * 1.44269504088896341f, -bits);
+            // 2^bits lifts the column's largest value to 2^22 or more and at most 127 2^16: three signed digits.
+            int bits = 0;
+            if (top > 0.f && top < __int_as_float(0x7F800000)) {
+                bits = min(22 - ilogbf(top), 126);
+                if (ldexpf(top, bits) > 8323072.f) --bits;
+            }
+            float f = ldexpf(a.scale * 1.44269504088896341f, -bits);
+            if (top == __int_as_float(0x7F800000)) f = __int_as_float(0x7FC00000);
+            const float up = ldexpf(1.f, bits);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                split_f16(x[4 * s] * up, x[4 * s + 1] * up, qh[nt][s][0], ql[nt][s][0]);
-                split_f16(x[4 * s + 2] * up, x[4 * s + 3] * up, qh[nt][s][1], ql[nt][s][1]);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    int v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = (__float2int_rn(x[8 * s + 4 * b + i] * up) + 0x8080) ^ 0x8080;
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) qd[nt][s][k][b] = byte_of(v, k);
+                }
             }
             factor[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
             factor[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
@@ -333,8 +371,11 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                 float sc[NT][MT][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
+                    int acc[NT][3][4];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) sc[nt][mt][0] = sc[nt][mt][1] = sc[nt][mt][2] = sc[nt][mt][3] = 0.f;
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) acc[nt][k][0] = acc[nt][k][1] = acc[nt][k][2] = acc[nt][k][3] = 0;
                     const int ra = mt * 16 + row_of(g);
 #pragma unroll
                     for (int c = 0; c < HD / 64; ++c) {
@@ -342,19 +383,22 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                         const int phys = HD == 128 ? (chunk ^ (ra & 7)) : (chunk ^ ((ra >> 1) & 3));
                         const uint4 wa = *reinterpret_cast<const uint4*>(kt + ra * HD + phys * 16);
                         const uint4 wb = *reinterpret_cast<const uint4*>(kt + (ra + 8) * HD + phys * 16);
-                        const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t xa = ua[i] ^ 0x80808080u, xb = ub[i] ^ 0x80808080u;
-                            const uint32_t a0 = codes_f16(xa, 0x4140), a2 = codes_f16(xa, 0x4342);
-                            const uint32_t a1 = codes_f16(xb, 0x4140), a3 = codes_f16(xb, 0x4342);
+                        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                mma_f16(sc[nt][mt], a0, a1, a2, a3, qh[nt][c * 4 + i][0], qh[nt][c * 4 + i][1]);
-                                mma_f16(sc[nt][mt], a0, a1, a2, a3, ql[nt][c * 4 + i][0], ql[nt][c * 4 + i][1]);
+                            for (int k = 0; k < 3; ++k) {
+                                mma_s8(acc[nt][k], wa.x, wb.x, wa.y, wb.y, qd[nt][2 * c][k][0], qd[nt][2 * c][k][1]);
+                                mma_s8(acc[nt][k], wa.z, wb.z, wa.w, wb.w, qd[nt][2 * c + 1][k][0], qd[nt][2 * c + 1][k][1]);
                             }
                         }
                     }
+                    // d0 + 256 d1 stays below 2^30, so one conversion takes both
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            sc[nt][mt][i] = fmaf(static_cast<float>(acc[nt][2][i]), 65536.f,
+                                                 static_cast<float>(acc[nt][1][i] * 256 + acc[nt][0][i]));
                 }
                 // Scores in exp2's units, masked; the online softmax of each column.
                 float keep[NT][2];
