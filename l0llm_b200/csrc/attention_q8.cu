@@ -154,16 +154,24 @@ __device__ __forceinline__ void team_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// Weights enter the MMA as hi + lo f16 terms, but for bf16 results: next to their rounding (2^-9 relative) that of a
+// weight to f16 (2^-12) is not seen, and 60 instructions a tile fall away.
+template <typename T>
+constexpr bool kWeightPairs = DT<T>::id != L0B_BF16;
+constexpr int kDigits = 3;  // of a query value
+
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __grid_constant__ Q8Launch L) {
     constexpr int W = warps_of(NT), COLS = 8 * NT;
     constexpr int SLOTS = kTileBytes / HD, MT = SLOTS / 16, HALVES = SLOTS / 32;
     constexpr int KS = HD / 32;   // 32-deep steps of K Q^T
     constexpr int DT_ = HD / 16;  // 16-dim tiles of O
+    constexpr int ND = kDigits;
+    constexpr bool PAIRS = kWeightPairs<T>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     long long* pre = reinterpret_cast<long long*>(ring + W * kStages * 2 * kTileBytes);
-    __shared__ __align__(8) uint64_t bars[W * kStages];
+    __shared__ __align__(8) uint64_t bars[W * kStages * 2];  // keys, values of each stage
     __shared__ float ml_s[W][COLS][2];
     __shared__ long long scan_s[W];
     __shared__ long long items_s;
@@ -173,7 +181,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     const Walk<NT> walk{a, pre, SLOTS};
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < W * kStages; ++i) bar_init(smem_addr(&bars[i]), 1);
+        for (int i = 0; i < W * kStages * 2; ++i) bar_init(smem_addr(&bars[i]), 1);
         bar_init_fence();
         items_s = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.kmap)) : "memory");
@@ -235,47 +243,67 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
 
     const int G = a.nh / a.nkv;
     uint8_t* my_ring = ring + warp * kStages * 2 * kTileBytes;
-    const uint32_t ring_addr = smem_addr(my_ring), bar_addr = smem_addr(&bars[warp * kStages]);
+    const uint32_t ring_addr = smem_addr(my_ring), bar_addr = smem_addr(&bars[warp * kStages * 2]);
 
-    // The fetching end of this warp's tile list: item, tile, and the scales of the two tiles in flight.
+    // The fetching end of this warp's tile list: item and tile, the scales of the two tiles in flight, and where the
+    // values of a tile whose keys alone are on their way start.
     Item fi = walk.find(u0);
-    int fj = static_cast<int>(u0 - fi.base) + wt;
+    int fj = static_cast<int>(u0 - fi.base) + wt, fend = 0;
+    const float *fks = nullptr, *fvs = nullptr;  // scales of the item's first block
+    auto enter = [&]() {
+        fend = static_cast<int>(min(static_cast<long long>(fi.tiles), u1 - fi.base));
+        const long long at = static_cast<long long>(fi.seq) * a.blocks * a.nkv + fi.head;
+        fks = a.ks + at;
+        fvs = a.vs + at;
+    };
     auto settle = [&]() {  // moves on to the item that holds the next tile; false at the end of the run
-        while (fj >= fi.tiles || fi.base + fj >= u1) {
+        while (fj >= fend) {
             if (fi.base + fi.tiles >= u1) return false;
             walk.next(fi);
             fj = wt;
+            enter();
         }
         return true;
     };
-    float ks_q[2][HALVES], vs_q[2][HALVES];  // [0]: the next tile to read, [1]: the one behind it
+    enter();
     const int block_log = 31 - __clz(a.block);
-    int issued = 0;
+    float ks_q[2][HALVES], vs_q[2][HALVES];  // [0]: the next tile to read, [1]: the one behind it
+    int issued = 0, vx = 0, vy = 0;
     bool more = settle();
-    auto fetch = [&](float (&ks)[HALVES], float (&vs)[HALVES]) {
+    auto fetch_keys = [&](float (&ks)[HALVES], float (&vs)[HALVES]) {
         const int st = issued & 1;
+        vx = fi.head * HD;
+        vy = fi.seq * a.max_seq + fj * SLOTS;
         if (lane == 0) {
-            const uint32_t bar = bar_addr + 8 * st, dst = ring_addr + st * 2 * kTileBytes;
-            bar_expect(bar, 2 * kTileBytes);
-            const int x = fi.head * HD, y = fi.seq * a.max_seq + fj * SLOTS;
-            tma_load(dst, &L.kmap, bar, x, y);
-            tma_load(dst + kTileBytes, &L.vmap, bar, x, y);
+            bar_expect(bar_addr + 16 * st, kTileBytes);
+            tma_load(ring_addr + st * 2 * kTileBytes, &L.kmap, bar_addr + 16 * st, vx, vy);
         }
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
             const int slot = fj * SLOTS + h * 32;
-            const long long at = (static_cast<long long>(fi.seq) * a.blocks + (slot >> block_log)) * a.nkv + fi.head;
+            const long long at = static_cast<long long>(slot >> block_log) * a.nkv;
             const bool holds = slot < fi.len;  // a block behind the sequence has no scale to speak of
-            ks[h] = holds ? __ldg(a.ks + at) : 0.f;
-            vs[h] = holds ? __ldg(a.vs + at) : 0.f;
+            ks[h] = holds ? __ldg(fks + at) : 0.f;
+            vs[h] = holds ? __ldg(fvs + at) : 0.f;
         }
         ++issued;
         fj += team_warps;
         more = settle();
     };
+    auto fetch_values = [&]() {
+        if (lane == 0) {
+            const int st = (issued - 1) & 1;
+            bar_expect(bar_addr + 16 * st + 8, kTileBytes);
+            tma_load(ring_addr + st * 2 * kTileBytes + kTileBytes, &L.vmap, bar_addr + 16 * st + 8, vx, vy);
+        }
+    };
     if (lane == 0) proxy_fence();
-    if (more) fetch(ks_q[0], vs_q[0]);
-    if (more) fetch(ks_q[1], vs_q[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (!more) break;
+        fetch_keys(ks_q[i], vs_q[i]);
+        fetch_values();
+    }
 
     int taken = 0;
     bool alive = true;  // false once a bounded wait gave up
@@ -288,7 +316,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
         const int cols = min(COLS, it.n * G - c0);
 
         // Query columns: lane (g, t) holds column nt * 8 + g, the dims that its key words will hold, as digits.
-        uint32_t qd[NT][KS][3][2];
+        uint32_t qd[NT][KS][ND][2];
         float factor[NT][2];  // score factor of this lane's accumulator columns nt * 8 + 2 t, + 1
         int seen[NT][2];      // slots those columns see
 #pragma unroll
@@ -314,7 +342,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             if (odd) top = __int_as_float(0x7F800000);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^bits lifts the column's largest value to 2^22 or more and at most 127 2^16: three signed digits.
+            // 2^bits lifts the column's largest value to 2^21 or more and at most 127 2^16: three signed digits.
             int bits = 0;
             if (top > 0.f && top < __int_as_float(0x7F800000)) {
                 bits = min(22 - ilogbf(top), 126);
@@ -331,7 +359,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[i] = (__float2int_rn(x[8 * s + 4 * b + i] * up) + 0x8080) ^ 0x8080;
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) qd[nt][s][k][b] = byte_of(v, k);
+                    for (int k = 0; k < ND; ++k) qd[nt][s][k][b] = byte_of(v, k);
                 }
             }
             factor[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
@@ -356,26 +384,36 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
         bool held = false;  // the stage of this warp's last tile of the segment, kept for the merge
         for (int j = j0 + wt; j < j1; j += team_warps) {
             const int st = taken & 1;
-            if (alive && !bar_wait(bar_addr + 8 * st, (taken >> 1) & 1)) {
-                alive = false;
-                if (lane == 0 && a.error) atomicOr(a.error, 1);
-            }
-            alive = __all_sync(0xffffffffu, alive);
+            const uint32_t parity = (taken >> 1) & 1;
+            // The last tile's stage stays as it is for the merge; any other's halves are filled again as they are read.
+            const bool refill = more && j + team_warps < j1;
+            auto wait = [&](uint32_t bar) {
+                if (alive && !bar_wait(bar, parity)) {
+                    alive = false;
+                    if (lane == 0 && a.error) atomicOr(a.error, 1);
+                }
+                alive = __all_sync(0xffffffffu, alive);
+            };
+            float ks_n[HALVES], vs_n[HALVES];  // scales of the tile fetched now
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) ks_n[h] = vs_n[h] = 0.f;
+            wait(bar_addr + 16 * st);
             const int first = j * SLOTS;
-            if (alive && first < seen_most) {
-                const uint8_t* kt = my_ring + st * 2 * kTileBytes;
-                const uint8_t* vt = kt + kTileBytes;
-                // Row r of a score tile is slot row_of(r) of its 16: an order in which the 16-byte reads of keys and
-                // of values below both touch every bank once.
-                auto row_of = [](int r) { return HD == 128 ? ((r >> 1) | ((r & 1) << 2)) : (r ^ ((r >> 1) & 1)); };
-                float sc[NT][MT][4];
+            const bool useful = alive && first < seen_most;
+            float sc[NT][MT][4];
+            // Row r of a score tile is slot row_of(r) of its 16: an order in which the 16-byte reads of keys and of
+            // values below both touch every bank once.
+            auto row_of = [](int r) { return HD == 128 ? ((r >> 1) | ((r & 1) << 2)) : (r ^ ((r >> 1) & 1)); };
+            const uint8_t* kt = my_ring + st * 2 * kTileBytes;
+            const uint8_t* vt = kt + kTileBytes;
+            if (useful) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    int acc[NT][3][4];
+                    int acc[NT][ND][4];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int k = 0; k < 3; ++k) acc[nt][k][0] = acc[nt][k][1] = acc[nt][k][2] = acc[nt][k][3] = 0;
+                        for (int k = 0; k < ND; ++k) acc[nt][k][0] = acc[nt][k][1] = acc[nt][k][2] = acc[nt][k][3] = 0;
                     const int ra = mt * 16 + row_of(g);
 #pragma unroll
                     for (int c = 0; c < HD / 64; ++c) {
@@ -386,7 +424,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                            for (int k = 0; k < 3; ++k) {
+                            for (int k = 0; k < ND; ++k) {
                                 mma_s8(acc[nt][k], wa.x, wb.x, wa.y, wb.y, qd[nt][2 * c][k][0], qd[nt][2 * c][k][1]);
                                 mma_s8(acc[nt][k], wa.z, wb.z, wa.w, wb.w, qd[nt][2 * c + 1][k][0], qd[nt][2 * c + 1][k][1]);
                             }
@@ -400,6 +438,10 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                             sc[nt][mt][i] = fmaf(static_cast<float>(acc[nt][2][i]), 65536.f,
                                                  static_cast<float>(acc[nt][1][i] * 256 + acc[nt][0][i]));
                 }
+            }
+            __syncwarp();  // every lane has read the keys
+            if (refill && alive) fetch_keys(ks_n, vs_n);
+            if (useful) {
                 // Scores in exp2's units, masked; the online softmax of each column.
                 float keep[NT][2];
                 bool grew = false;
@@ -453,6 +495,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                         }
                     }
                 }
+                wait(bar_addr + 16 * st + 8);
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h) {
                     if (first + h * 32 >= seen_most) break;
@@ -468,7 +511,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
 #pragma unroll
                             for (int b = 0; b < 2; ++b) {
                                 ph[nt][k][b] = transposed(ph[nt][k][b]);
-                                pl[nt][k][b] = transposed(pl[nt][k][b]);
+                                if constexpr (PAIRS) pl[nt][k][b] = transposed(pl[nt][k][b]);
                             }
                         }
                         // a column that sees none of these slots takes nothing of their scale, whatever it is
@@ -517,7 +560,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) {
                                     mma_f16(acc[d][nt], a0, a1, a2, a3, ph[nt][k][0], ph[nt][k][1]);
-                                    mma_f16(acc[d][nt], a0, a1, a2, a3, pl[nt][k][0], pl[nt][k][1]);
+                                    if constexpr (PAIRS) mma_f16(acc[d][nt], a0, a1, a2, a3, pl[nt][k][0], pl[nt][k][1]);
                                 }
                             }
                         }
@@ -535,17 +578,17 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                     }
                 }
             }
+            if (!useful) wait(bar_addr + 16 * st + 8);
             ++taken;
+            __syncwarp();  // every lane has read the values
+            if (refill && alive) fetch_values();
+            if (!(j + team_warps < j1)) held = true;
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
                 ks_q[0][h] = ks_q[1][h];
                 vs_q[0][h] = vs_q[1][h];
-            }
-            __syncwarp();  // every lane has read the stage
-            if (j + team_warps < j1) {
-                if (more && alive) fetch(ks_q[1], vs_q[1]);
-            } else {
-                held = true;
+                ks_q[1][h] = ks_n[h];
+                vs_q[1][h] = vs_n[h];
             }
         }
 
@@ -669,13 +712,17 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
         team_sync(bar_id, team_warps * 32);  // the dumps are read: their stages may be filled again
         if (held && more && alive) {
             if (lane == 0) proxy_fence();
-            fetch(ks_q[1], vs_q[1]);
+            fetch_keys(ks_q[1], vs_q[1]);
+            fetch_values();
         }
         walk.next(it);
     }
     // A warp that gave up leaves no copy of its own in flight behind it.
     if (!alive) {
-        for (; taken < issued; ++taken) bar_wait(bar_addr + 8 * (taken & 1), (taken >> 1) & 1);
+        for (; taken < issued; ++taken) {
+            bar_wait(bar_addr + 16 * (taken & 1), (taken >> 1) & 1);
+            bar_wait(bar_addr + 16 * (taken & 1) + 8, (taken >> 1) & 1);
+        }
     }
 }
 
