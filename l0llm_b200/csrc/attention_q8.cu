@@ -1,8 +1,11 @@
 // Attention over the int8 KV cache (sm_100a, mma.sync m16n8k16 with f32 accumulators, TMA-fed).
 //
-// The work is flat: for every (sequence, KV head, group of query columns) -- an item -- its tiles of 4 KB of keys
-// and 4 KB of values (32 slots of head dim 128, 64 of 64), in order. Each of N teams of warps takes an equal run of
-// that list, whatever the mix of lengths, which the kernel reads on the device; one launch, one CTA per SM. A run
+// The work is flat: for every (sequence, group of query columns) -- an item -- its tiles of 4 KB of keys and 4 KB of
+// values (32 slots of head dim 128, 64 of 64), in order: one list, the same for every KV head. A group of teams of
+// warps, one team per head, takes an equal run of that list, whatever the mix of lengths, which the kernel reads on
+// the device; one launch, one CTA per SM. So the teams that run side by side read the heads of the same slots, whole
+// cache rows, at the same time: with each head's list split on its own (hd bytes out of every row) the DRAM pages
+// were opened once per head, and 1.05 GB of 8 heads took 283 us where the same bytes of one head took 178. A run
 // crosses items: the part of it inside one item is a segment. A warp takes every TEAM-th tile of its team's segment,
 // fetched by its own TMA two tiles ahead, segments ahead included, so HBM stays busy through their ends.
 //
@@ -19,8 +22,8 @@
 // Softmax online, per warp and column, in exp2; weights carry a factor 2^14 that keeps their lo terms normal f16.
 //
 // At a segment's end the team's warps meet in shared memory (each in the ring stage it has just read). An item that
-// several teams share has its parts joined, in team order, by the team that arrives last (a counter per first team,
-// which that team resets), so results do not depend on the order of arrival.
+// several groups share has its parts joined, in group order, by the team that arrives last (a counter per first team,
+// which the joining team resets), so results do not depend on the order of arrival.
 //
 // Bound by HBM for long contexts (2 hd bytes a slot and KV head), by latency for short ones.
 #include <mutex>
@@ -50,8 +53,7 @@ struct Q8Launch {
 
 // What a warp needs to know of one item, and the walk over items.
 struct Item {
-    int seq;            // sequence
-    int head, cg;       // KV head, column group
+    int seq, cg;        // sequence, column group
     int cgroups;        // column groups of the sequence
     int tiles;
     int len, n, row0;   // slots held, query rows, first packed row
@@ -88,18 +90,14 @@ struct Walk {
         Item it;
         it.seq = lo;
         load_sequence(it);
-        const int sub = static_cast<int>((u - pre[lo]) / it.tiles);
-        it.head = sub / it.cgroups;
-        it.cg = sub - it.head * it.cgroups;
-        it.base = pre[lo] + static_cast<long long>(sub) * it.tiles;
+        it.cg = static_cast<int>((u - pre[lo]) / it.tiles);
+        it.base = pre[lo] + static_cast<long long>(it.cg) * it.tiles;
         return it;
     }
     __device__ __forceinline__ void next(Item& it) const {
         it.base += it.tiles;
         if (++it.cg < it.cgroups) return;
         it.cg = 0;
-        if (++it.head < a.nkv) return;
-        it.head = 0;
         do ++it.seq;
         while (it.seq + 1 < a.count && pre[it.seq] == pre[it.seq + 1]);
         if (it.seq < a.count) load_sequence(it);
@@ -200,9 +198,8 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             if (blockIdx.x == 0 && (__ldg(a.lengths + i) != len ||
                                     (a.starts && (__ldg(a.starts + i) < 0 || __ldg(a.starts + i + 1) > a.tokens))))
                 flag_bad_index(a.error);
-            const long long subs = static_cast<long long>(walk.column_groups(n)) * a.nkv;
-            units += subs * walk.tiles_of(len);
-            items += subs;
+            units += static_cast<long long>(walk.column_groups(n)) * walk.tiles_of(len);
+            items += walk.column_groups(n);
         }
         long long sum = units;
 #pragma unroll
@@ -221,7 +218,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             int row0, n, len;
             walk.sequence(i, row0, n, len);
             pre[i] = before;
-            before += static_cast<long long>(walk.column_groups(n)) * a.nkv * walk.tiles_of(len);
+            before += static_cast<long long>(walk.column_groups(n)) * walk.tiles_of(len);
         }
         if (threadIdx.x == 0) {
             long long all = 0;
@@ -235,16 +232,22 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     // two rounds of the CTA's warps): teams of four, so that more items are worked on at once.
     const int team_warps = U >= 2 * W * items_s ? W : 4;
     const int teams = W / team_warps;
-    const int N = static_cast<int>(min(U, static_cast<long long>(gridDim.x * teams)));  // every team has a unit or more
     const int tid = threadIdx.x % (team_warps * 32), wt = warp % team_warps, local = warp / team_warps;
     const int team = local * gridDim.x + blockIdx.x;
-    if (team >= N) return;
-    const long long u0 = U * team / N, u1 = U * (team + 1) / N;
+    // Heads at a time (all, but where they outnumber the teams), and N groups of that many teams; every group has a
+    // unit or more. Heads that wait for a second turn are then of one group, which shares no item.
+    const int heads = min(a.nkv, static_cast<int>(gridDim.x) * teams);
+    const int N = static_cast<int>(min(U, static_cast<long long>(gridDim.x * teams / heads)));
+    const int group = team / heads;
+    if (group >= N) return;
+    const long long u0 = U * group / N, u1 = U * (group + 1) / N;
 
     const int G = a.nh / a.nkv;
+    int issued = 0, taken = 0;  // tiles of this warp
+    bool alive = true;          // false once a bounded wait gave up
     uint8_t* my_ring = ring + warp * kStages * 2 * kTileBytes;
     const uint32_t ring_addr = smem_addr(my_ring), bar_addr = smem_addr(&bars[warp * kStages * 2]);
-
+    for (int kvh = team - group * heads; kvh < a.nkv; kvh += heads) {
     // The fetching end of this warp's tile list: item and tile, the scales of the two tiles in flight, and where the
     // values of a tile whose keys alone are on their way start.
     Item fi = walk.find(u0);
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     const float *fks = nullptr, *fvs = nullptr;  // scales of the item's first block
     auto enter = [&]() {
         fend = static_cast<int>(min(static_cast<long long>(fi.tiles), u1 - fi.base));
-        const long long at = static_cast<long long>(fi.seq) * a.blocks * a.nkv + fi.head;
+        const long long at = static_cast<long long>(fi.seq) * a.blocks * a.nkv + kvh;
         fks = a.ks + at;
         fvs = a.vs + at;
     };
@@ -268,11 +271,11 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     enter();
     const int block_log = 31 - __clz(a.block);
     float ks_q[2][HALVES], vs_q[2][HALVES];  // [0]: the next tile to read, [1]: the one behind it
-    int issued = 0, vx = 0, vy = 0;
+    int vx = 0, vy = 0;
     bool more = settle();
     auto fetch_keys = [&](float (&ks)[HALVES], float (&vs)[HALVES]) {
         const int st = issued & 1;
-        vx = fi.head * HD;
+        vx = kvh * HD;
         vy = fi.seq * a.max_seq + fj * SLOTS;
         if (lane == 0) {
             bar_expect(bar_addr + 16 * st, kTileBytes);
@@ -305,14 +308,12 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
         fetch_values();
     }
 
-    int taken = 0;
-    bool alive = true;  // false once a bounded wait gave up
     long long u = u0;
     Item it = walk.find(u0);
     while (true) {
         const int j0 = static_cast<int>(u - it.base);
         const int j1 = static_cast<int>(min(static_cast<long long>(it.tiles), u1 - it.base));
-        const int kvh = it.head, c0 = it.cg * COLS;  // first column
+        const int c0 = it.cg * COLS;  // first column
         const int cols = min(COLS, it.n * G - c0);
 
         // Query columns: lane (g, t) holds column nt * 8 + g, the dims that its key words will hold, as digits.
@@ -632,7 +633,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
         const int w0 = local * team_warps;
         const bool whole = j0 == 0 && j1 == it.tiles;
         const int ta = static_cast<int>(((it.base + 1) * N - 1) / U), tb = static_cast<int>(((it.base + it.tiles) * N - 1) / U);
-        const long long slot = 2LL * team + (team == ta ? 1 : 0);
+        const long long slot = 2LL * team + (group == ta ? 1 : 0);
         for (int e = tid; e < cols * (HD / 4); e += team_warps * 32) {
             const int c = e / (HD / 4), x = e - c * (HD / 4);
             float top = kNegInf;
@@ -669,8 +670,9 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             __threadfence();
             team_sync(bar_id, team_warps * 32);
             if (tid == 0) {
-                const bool last = atomicAdd(&L.counters[ta], 1u) == static_cast<unsigned>(tb - ta);
-                if (last) L.counters[ta] = 0;
+                unsigned* arrived = &L.counters[ta * heads + kvh];
+                const bool last = atomicAdd(arrived, 1u) == static_cast<unsigned>(tb - ta);
+                if (last) *arrived = 0;
                 __threadfence();
                 last_s[w0] = last ? 2u : 3u;
             }
@@ -681,11 +683,11 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                     const int c = e / (HD / 4), x = e - c * (HD / 4);
                     float top = kNegInf;
                     for (int k = ta; k <= tb; ++k)
-                        top = fmaxf(top, __ldcg(L.part_ml + ((2LL * k + (k == ta)) * COLS + c) * 2));
+                        top = fmaxf(top, __ldcg(L.part_ml + ((2LL * (k * heads + kvh) + (k == ta)) * COLS + c) * 2));
                     float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
                     for (int k = ta; k <= tb; ++k) {
-                        const long long s = (2LL * k + (k == ta)) * COLS + c;
+                        const long long s = (2LL * (k * heads + kvh) + (k == ta)) * COLS + c;
                         const float2 ml = __ldcg(reinterpret_cast<const float2*>(L.part_ml + s * 2));
                         const float4 y = __ldcg(reinterpret_cast<const float4*>(L.part + s * HD + x * 4));
                         const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - top);
@@ -716,6 +718,8 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             fetch_values();
         }
         walk.next(it);
+    }
+    team_sync(1 + local, team_warps * 32);
     }
     // A warp that gave up leaves no copy of its own in flight behind it.
     if (!alive) {
