@@ -296,7 +296,7 @@ L0B_API l0b_status l0b_attention_execute_packed(l0b_suite* s, l0b_device* d, l0b
  * call is row i of these buffers (l0b_buffer_view names a run of rows). All zero (as allocated) is a valid empty
  * cache. starts: i32 [count + 1], the packed rows of each sequence as in l0b_attention_execute_packed; NULL: one
  * row a sequence (tokens == count). positions / lengths: i32 [count]. All are read on the device, so a recorded
- * command list follows their contents. hd 64 or 128; count <= 4096.
+ * command list follows their contents; starts ascend. hd 64 or 128; count <= 4096.
  *
  * Store: rows of k / v [tokens, nKv * hd] (f32, f16 or bf16, row strides as above) go to slots positions[i],
  * positions[i] + 1, ... The scale of a block is f32(max|x| / 127) over its new rows and the codes are

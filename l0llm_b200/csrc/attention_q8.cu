@@ -52,18 +52,22 @@ struct Q8Launch {
 };
 
 // What a warp needs to know of one item, and the walk over items.
+// An item takes kItemUnits units and one for each of its tiles: starting and ending one costs as much as some twenty
+// tiles (query digits, the joining of states; 4 us of latency), and runs of equal length would be uneven without it.
+constexpr int kItemUnits = 20;
+
 struct Item {
-    int seq, cg;        // sequence, column group
-    int cgroups;        // column groups of the sequence
+    int seq, cg;       // sequence, column group
+    int cgroups;       // column groups of the sequence
     int tiles;
-    int len, n, row0;   // slots held, query rows, first packed row
-    long long base;     // first unit
+    int len, n, row0;  // slots held, query rows, first packed row
+    int base;          // unit of the first tile
 };
 
 template <int NT>
 struct Walk {
     const AttnQ8Params& a;
-    const long long* pre;
+    const int* pre;  // units before each sequence
     int slots;  // per tile
 
     __device__ __forceinline__ void sequence(int i, int& row0, int& n, int& len) const {
@@ -79,8 +83,10 @@ struct Walk {
         it.cgroups = column_groups(it.n);
         it.tiles = tiles_of(it.len);
     }
+    // Units of a sequence of n rows and len slots.
+    __device__ __forceinline__ int units(int n, int len) const { return column_groups(n) * (kItemUnits + tiles_of(len)); }
     // The item that holds unit u.
-    __device__ __forceinline__ Item find(long long u) const {
+    __device__ __forceinline__ Item find(int u) const {
         int lo = 0, hi = a.count;  // pre[lo] <= u < pre[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -90,12 +96,12 @@ struct Walk {
         Item it;
         it.seq = lo;
         load_sequence(it);
-        it.cg = static_cast<int>((u - pre[lo]) / it.tiles);
-        it.base = pre[lo] + static_cast<long long>(it.cg) * it.tiles;
+        it.cg = (u - pre[lo]) / (kItemUnits + it.tiles);
+        it.base = pre[lo] + it.cg * (kItemUnits + it.tiles) + kItemUnits;
         return it;
     }
     __device__ __forceinline__ void next(Item& it) const {
-        it.base += it.tiles;
+        it.base += it.tiles + kItemUnits;
         if (++it.cg < it.cgroups) return;
         it.cg = 0;
         do ++it.seq;
@@ -168,11 +174,11 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     constexpr bool PAIRS = kWeightPairs<T>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    long long* pre = reinterpret_cast<long long*>(ring + W * kStages * 2 * kTileBytes);
+    int* pre = reinterpret_cast<int*>(ring + W * kStages * 2 * kTileBytes);
     __shared__ __align__(8) uint64_t bars[W * kStages * 2];  // keys, values of each stage
     __shared__ float ml_s[W][COLS][2];
-    __shared__ long long scan_s[W];
-    __shared__ long long items_s;
+    __shared__ int scan_s[W][2];
+    __shared__ unsigned long long rows_s;
     __shared__ unsigned last_s[W];
     const AttnQ8Params& a = L.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -181,7 +187,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     if (threadIdx.x == 0) {
         for (int i = 0; i < W * kStages * 2; ++i) bar_init(smem_addr(&bars[i]), 1);
         bar_init_fence();
-        items_s = 0;
+        rows_s = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.kmap)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.vmap)) : "memory");
     }
@@ -191,56 +197,79 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     // pre[i] = units before sequence i: every CTA scans the lengths (a few loads a thread).
     {
         const int per = (a.count + W * 32 - 1) / (W * 32), i0 = threadIdx.x * per, i1 = min(a.count, i0 + per);
-        long long units = 0, items = 0;
+        int units = 0, items = 0;
+        long long rows = 0;
         for (int i = i0; i < i1; ++i) {
             int row0, n, len;
             walk.sequence(i, row0, n, len);
             if (blockIdx.x == 0 && (__ldg(a.lengths + i) != len ||
                                     (a.starts && (__ldg(a.starts + i) < 0 || __ldg(a.starts + i + 1) > a.tokens))))
                 flag_bad_index(a.error);
-            units += static_cast<long long>(walk.column_groups(n)) * walk.tiles_of(len);
+            units += walk.units(n, len);
             items += walk.column_groups(n);
+            rows += n;
         }
-        long long sum = units;
+        int sum = units;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += up;
-            items += __shfl_xor_sync(0xffffffffu, items, o);
         }
+        items = __reduce_add_sync(0xffffffffu, items);
         __syncthreads();
-        if (lane == 31) scan_s[warp] = sum;
-        if (lane == 0 && items) atomicAdd(reinterpret_cast<unsigned long long*>(&items_s), static_cast<unsigned long long>(items));
+        if (lane == 31) {
+            scan_s[warp][0] = sum;
+            scan_s[warp][1] = items;
+        }
+        if (rows) atomicAdd(&rows_s, static_cast<unsigned long long>(rows));
         __syncthreads();
-        long long before = sum - units;
-        for (int w = 0; w < warp; ++w) before += scan_s[w];
+        if (rows_s > static_cast<unsigned long long>(a.tokens)) {  // starts that descend name rows more than once
+            if (threadIdx.x == 0) flag_bad_index(a.error);
+            return;
+        }
+        int before = sum - units;
+        for (int w = 0; w < warp; ++w) before += scan_s[w][0];
         for (int i = i0; i < i1; ++i) {
             int row0, n, len;
             walk.sequence(i, row0, n, len);
             pre[i] = before;
-            before += static_cast<long long>(walk.column_groups(n)) * walk.tiles_of(len);
+            before += walk.units(n, len);
         }
         if (threadIdx.x == 0) {
-            long long all = 0;
-            for (int w = 0; w < W; ++w) all += scan_s[w];
+            int all = 0;
+            for (int w = 0; w < W; ++w) all += scan_s[w][0];
             pre[a.count] = all;
         }
         __syncthreads();
     }
-    const long long U = pre[a.count];
+    const int U = pre[a.count];
+    if (U == 0) return;
     // Long items: the CTA's warps share one run, which has the fewest parts to join. Short items (fewer tiles than
     // two rounds of the CTA's warps): teams of four, so that more items are worked on at once.
-    const int team_warps = U >= 2 * W * items_s ? W : 4;
+    int items = 0;
+    for (int w = 0; w < W; ++w) items += scan_s[w][1];
+    const int team_warps = U >= static_cast<long long>(2 * W + kItemUnits) * items ? W : 4;
     const int teams = W / team_warps;
     const int tid = threadIdx.x % (team_warps * 32), wt = warp % team_warps, local = warp / team_warps;
     const int team = local * gridDim.x + blockIdx.x;
-    // Heads at a time (all, but where they outnumber the teams), and N groups of that many teams; every group has a
-    // unit or more. Heads that wait for a second turn are then of one group, which shares no item.
+    // Heads at a time (all, but where they outnumber the teams), and N groups of that many teams, each with an equal
+    // run of units. Heads that wait for a second turn are then of one group, which shares no item.
     const int heads = min(a.nkv, static_cast<int>(gridDim.x) * teams);
-    const int N = static_cast<int>(min(U, static_cast<long long>(gridDim.x * teams / heads)));
+    const int N = min(U, static_cast<int>(gridDim.x) * teams / heads);
     const int group = team / heads;
     if (group >= N) return;
-    const long long u0 = U * group / N, u1 = U * (group + 1) / N;
+    const int run = U / N, over = U - run * N;
+    auto start_of = [&](int k) { return run * k + over * k / N; };
+    auto group_of = [&](int u) {  // the last k with start_of(k) <= u
+        int lo = 0, hi = N;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start_of(mid) <= u) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    const int u0 = start_of(group), u1 = start_of(group + 1);
 
     const int G = a.nh / a.nkv;
     int issued = 0, taken = 0;  // tiles of this warp
@@ -251,17 +280,17 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     // The fetching end of this warp's tile list: item and tile, the scales of the two tiles in flight, and where the
     // values of a tile whose keys alone are on their way start.
     Item fi = walk.find(u0);
-    int fj = static_cast<int>(u0 - fi.base) + wt, fend = 0;
+    int fj = max(0, u0 - fi.base) + wt, fend = 0;
     const float *fks = nullptr, *fvs = nullptr;  // scales of the item's first block
     auto enter = [&]() {
-        fend = static_cast<int>(min(static_cast<long long>(fi.tiles), u1 - fi.base));
+        fend = min(fi.tiles, u1 - fi.base);
         const long long at = static_cast<long long>(fi.seq) * a.blocks * a.nkv + kvh;
         fks = a.ks + at;
         fvs = a.vs + at;
     };
     auto settle = [&]() {  // moves on to the item that holds the next tile; false at the end of the run
         while (fj >= fend) {
-            if (fi.base + fi.tiles >= u1) return false;
+            if (fi.base + fi.tiles + kItemUnits >= u1) return false;
             walk.next(fi);
             fj = wt;
             enter();
@@ -308,11 +337,9 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
         fetch_values();
     }
 
-    long long u = u0;
     Item it = walk.find(u0);
-    while (true) {
-        const int j0 = static_cast<int>(u - it.base);
-        const int j1 = static_cast<int>(min(static_cast<long long>(it.tiles), u1 - it.base));
+    while (it.base < u1) {  // a run may end before the first tile of its last item
+        const int j0 = max(0, u0 - it.base), j1 = min(it.tiles, u1 - it.base);
         const int c0 = it.cg * COLS;  // first column
         const int cols = min(COLS, it.n * G - c0);
 
@@ -632,7 +659,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
         team_sync(bar_id, team_warps * 32);
         const int w0 = local * team_warps;
         const bool whole = j0 == 0 && j1 == it.tiles;
-        const int ta = static_cast<int>(((it.base + 1) * N - 1) / U), tb = static_cast<int>(((it.base + it.tiles) * N - 1) / U);
+        const int ta = whole ? group : group_of(it.base), tb = whole ? group : group_of(it.base + it.tiles - 1);
         const long long slot = 2LL * team + (group == ta ? 1 : 0);
         for (int e = tid; e < cols * (HD / 4); e += team_warps * 32) {
             const int c = e / (HD / 4), x = e - c * (HD / 4);
@@ -709,8 +736,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                 }
             }
         }
-        u = it.base + j1;
-        if (u >= u1) break;
+        if (it.base + it.tiles + kItemUnits >= u1) break;
         team_sync(bar_id, team_warps * 32);  // the dumps are read: their stages may be filled again
         if (held && more && alive) {
             if (lane == 0) proxy_fence();
@@ -741,10 +767,14 @@ l0b_status launch_q8(l0b_suite* s, l0b_device* d, const AttnQ8Params& a) {
         std::lock_guard<std::mutex> lock(mu);
         if (d->index >= 64 || !configured[d->index]) {
             L0B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                static_cast<int>(ring + 8 * (kMaxSequences + 1))));
+                                                static_cast<int>(ring + 4 * (kMaxSequences + 1))));
             if (d->index < 64) configured[d->index] = true;
         }
     }
+    // Units are counted in 32 bits: rows of a call times tiles of a cache row, at worst.
+    const long long groups = (static_cast<long long>(a.tokens) * (a.nh / a.nkv)) / (8 * NT) + a.count;
+    L0B_REQUIRE(groups <= INT32_MAX / (a.max_seq / (kTileBytes / HD) + 1 + kItemUnits), L0B_ERR_OUT_OF_RANGE,
+                "%d query rows against %d slots are too many for one call", a.tokens, a.max_seq);
     Q8Launch L;
     std::memset(&L, 0, sizeof L);
     const long long rows = static_cast<long long>(a.count) * a.max_seq, width = static_cast<long long>(a.nkv) * HD;
@@ -755,7 +785,7 @@ l0b_status launch_q8(l0b_suite* s, l0b_device* d, const AttnQ8Params& a) {
     L.part = s->q8_part;
     L.part_ml = s->q8_part + static_cast<size_t>(2 * kQ8TeamsPerSm) * d->sm_count * 16 * 128;
     L.counters = s->q8_counters;
-    return d->launch(kernel, dim3(d->sm_count), dim3(W * 32), ring + 8 * (static_cast<size_t>(a.count) + 1), L);
+    return d->launch(kernel, dim3(d->sm_count), dim3(W * 32), ring + 4 * (static_cast<size_t>(a.count) + 1), L);
 }
 
 template <typename T>
