@@ -253,9 +253,11 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     const int tid = threadIdx.x % (team_warps * 32), wt = warp % team_warps, local = warp / team_warps;
     const int team = local * gridDim.x + blockIdx.x;
     // Heads at a time (all, but where they outnumber the teams), and N groups of that many teams, each with an equal
-    // run of units. Heads that wait for a second turn are then of one group, which shares no item.
+    // run of units: of a tile a warp or more, since parts cost more to join than idle warps. Heads that wait for a
+    // second turn are of one group, which shares no item.
     const int heads = min(a.nkv, static_cast<int>(gridDim.x) * teams);
-    const int N = min(U, static_cast<int>(gridDim.x) * teams / heads);
+    const int tiles = U - items * kItemUnits;
+    const int N = min((tiles + team_warps - 1) / team_warps, static_cast<int>(gridDim.x) * teams / heads);
     const int group = team / heads;
     if (group >= N) return;
     const int run = U / N, over = U - run * N;
@@ -694,9 +696,9 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             }
         }
         if (!whole) {
-            __threadfence();
             team_sync(bar_id, team_warps * 32);
             if (tid == 0) {
+                __threadfence();  // after the barrier: for the whole team's writes
                 unsigned* arrived = &L.counters[ta * heads + kvh];
                 const bool last = atomicAdd(arrived, 1u) == static_cast<unsigned>(tb - ta);
                 if (last) *arrived = 0;

@@ -7,14 +7,15 @@ import numpy as np
 def attention(q, k, v, position, heads, kv_heads):
     """q [n, heads * hd], k / v [m, kv_heads * hd] as f64 values, position [n]: query t sees keys [0, position[t]].
 
-    Returns out [n, heads, hd], spread = sqrt(sum_j (p_j v_j)^2) of each output, and dot [n, heads] = the largest
-    sum_i |q_i k_i| / sqrt(hd) over the keys of a row (what a score's rounding errors are relative to)."""
+    Returns out [n, heads, hd], spread = sqrt(sum_j (p_j v_j)^2) of each output, dot [n, heads] = the largest
+    sum_i |q_i k_i| / sqrt(hd) over the keys of a row (what a score's rounding errors are relative to), and mass
+    [n, heads, hd] = sum_j |v_j|."""
     n, m = q.shape[0], k.shape[0]
     hd = q.shape[1] // heads
     q = q.reshape(n, heads, hd).astype(np.float64)
     k = k.reshape(m, kv_heads, hd).astype(np.float64)
     v = v.reshape(m, kv_heads, hd).astype(np.float64)
-    out, spread, dot = np.zeros((n, heads, hd)), np.zeros((n, heads, hd)), np.zeros((n, heads))
+    out, spread, mass, dot = (np.zeros((n, heads, hd)[:k]) for k in (3, 3, 3, 2))
     group = heads // kv_heads
     for t in range(n):
         reach = min(int(position[t]) + 1, m)
@@ -27,11 +28,12 @@ def attention(q, k, v, position, heads, kv_heads):
             p /= p.sum()
             out[t, h] = p @ vv
             spread[t, h] = np.sqrt((p * p) @ (vv * vv))
+            mass[t, h] = np.abs(vv).sum(0)
             dot[t, h] = np.abs(kk * q[t, h]).sum(1).max() / np.sqrt(hd)
-    return out, spread, dot
+    return out, spread, dot, mass
 
 
-def attention_bound(out, spread, dot, hd, unit_p, unit_out):
+def attention_bound(out, spread, dot, mass, hd, unit_p, unit_out, floor_p=2.0 ** -38):
     """How far a kernel's out may be off, from the arithmetic:
 
     - a probability rounded by at most unit_p moves an output by a sum of independent terms, each at most unit_p p_j
@@ -40,10 +42,12 @@ def attention_bound(out, spread, dot, hd, unit_p, unit_out):
       operand split) is off by at most (hd / 8 + 4) 2^-23 dot, and an exp2 of it by 2^-22 more; the same factor on
       every weight cancels, so half the range counts, on terms of random sign: again 8 spread;
     - sums of weights and of values in f32, rescaled from tile to tile: 64 steps of 2^-23 of the output, and of spread;
+    - a weight in f16 has steps of 2^-24 at least, where weights are held under a factor 2^14 that is half a step of
+      2^-39 of the largest for each of two terms: floor_p of it on every value, however small its weight;
     - the result's own rounding, unit_out relative."""
     f32 = 2.0 ** -23
     score = (hd / 8 + 4) * f32 * dot[..., None] + 2 * f32
-    return 8 * spread * (unit_p + score) + 64 * f32 * (np.abs(out) + spread) + unit_out * np.abs(out) + 1e-30
+    return 8 * spread * (unit_p + score) + 64 * f32 * (np.abs(out) + spread) + unit_out * np.abs(out) + floor_p * mass + 1e-30
 
 
 def codes_of(x, scale):

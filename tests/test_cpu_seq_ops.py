@@ -46,6 +46,6 @@ def test_store_keeps_values_within_half_a_step_of_each_store(block):
 def test_attention_with_nothing_to_see_is_zero():
     rng = np.random.default_rng(1)
     q, k = rng.standard_normal((5, 4 * 64)), rng.standard_normal((3, 2 * 64))
-    out, spread, _ = so.attention(q, k, k, np.arange(-2, 3), 4, 2)
+    out, spread, *_ = so.attention(q, k, k, np.arange(-2, 3), 4, 2)
     assert not out[:2].any() and np.all(out[2] == k[0].reshape(2, 64).repeat(2, 0))
     np.testing.assert_allclose(spread[2], np.abs(out[2]))

@@ -222,8 +222,8 @@ def attend(lz, device, suite, c, nh, n, lengths, dt, seed=0, starts="sum", gain=
     for i, (m, length) in enumerate(zip(n, lengths)):
         k, v = (so.values(c.codes[w][i][:length], c.scales[w][i], c.block).reshape(length, c.nkv * c.hd)
             for w in range(2))
-        o, spread, dot = so.attention(qv[a:a + m], k, v, np.arange(length - m, length), nh, c.nkv)
-        want[a:a + m], bound[a:a + m] = o, so.attention_bound(o, spread, dot, c.hd, UNIT_P[dt], UNIT[dt])
+        o, *errs = so.attention(qv[a:a + m], k, v, np.arange(length - m, length), nh, c.nkv)
+        want[a:a + m], bound[a:a + m] = o, so.attention_bound(o, *errs, c.hd, UNIT_P[dt], UNIT[dt])
         a += m
     return got, want, bound
 
@@ -520,8 +520,8 @@ def test_prompts_stored_decoded_and_continued(lz, device, suite):
     for i, n in enumerate(prompt):
         a = slice(starts[i], starts[i + 1])
         kk, vv = (from_type(as_type(x[a], "f16")[0], "f16") for x in (k, v))
-        o, spread, dot = so.attention(q[a], kk, vv, np.arange(n), nh, nkv)
-        assert_within(got[a], o, so.attention_bound(o, spread, dot, hd, UNIT_P["f32"], UNIT["f32"]))
+        o, *errs = so.attention(q[a], kk, vv, np.arange(n), nh, nkv)
+        assert_within(got[a], o, so.attention_bound(o, *errs, hd, UNIT_P["f32"], UNIT["f32"]))
     # decode: the same list each step, positions and lengths written before it
     lengths = np.array(prompt, np.int32)
     po, le = c.int_buffer(lengths), c.int_buffer(lengths + 1)
@@ -544,8 +544,8 @@ def test_prompts_stored_decoded_and_continued(lz, device, suite):
             for i in range(3):
                 kk, vv = (so.values(c.codes[w][i][:lengths[i]], c.scales[w][i], block).reshape(lengths[i], -1)
                           for w in range(2))
-                o, spread, dot = so.attention(x[2][i:i + 1], kk, vv, [lengths[i] - 1], nh, nkv)
-                assert_within(got[i:i + 1], o, so.attention_bound(o, spread, dot, hd, UNIT_P["f32"], UNIT["f32"]))
+                o, *errs = so.attention(x[2][i:i + 1], kk, vv, [lengths[i] - 1], nh, nkv)
+                assert_within(got[i:i + 1], o, so.attention_bound(o, *errs, hd, UNIT_P["f32"], UNIT["f32"]))
     # continue: load what is cached in front of new rows, in one packed buffer
     new = [20, 9, 33]
     total = [int(a + b) for a, b in zip(lengths, new)]
@@ -575,8 +575,8 @@ def test_prompts_stored_decoded_and_continued(lz, device, suite):
         cached = so.values(c.codes[0][i][:lengths[i]], c.scales[0][i], block).reshape(lengths[i], -1)
         np.testing.assert_array_equal(kk[ks[i]:ks[i] + lengths[i]], cached.astype(np.float32).astype(np.float16))
         a, b = slice(ns[i], ns[i + 1]), slice(ks[i], ks[i + 1])
-        o, spread, dot = so.attention(nq[a], kk[b], vv[b], np.arange(total[i] - new[i], total[i]), nh, nkv)
-        assert_within(got[a], o, so.attention_bound(o, spread, dot, hd, UNIT_P["f32"], UNIT["f32"]))
+        o, *errs = so.attention(nq[a], kk[b], vv[b], np.arange(total[i] - new[i], total[i]), nh, nkv)
+        assert_within(got[a], o, so.attention_bound(o, *errs, hd, UNIT_P["f32"], UNIT["f32"]))
     assert status(lz, device) == 0
     for x in (st, zero, po, le, tk, tv, tq, to, ka, va, qn, on, stn, stk, *bufs.values()):
         x.Dispose()

@@ -82,18 +82,18 @@ class Packed:
         return got
 
     def want(self):
-        out, spread = (np.zeros((self.tokens, self.nh, self.hd)) for _ in range(2))
+        out, spread, mass = (np.zeros((self.tokens, self.nh, self.hd)) for _ in range(3))
         dot = np.zeros((self.tokens, self.nh))
         for i, (n, m) in enumerate(zip(self.n, self.m)):
             a, b = self.q_starts[i], self.kv_starts[i]
-            out[a:a + n], spread[a:a + n], dot[a:a + n] = so.attention(
+            out[a:a + n], spread[a:a + n], dot[a:a + n], mass[a:a + n] = so.attention(
                 self.qv[a:a + n], self.kv[b:b + m], self.vv[b:b + m], np.arange(m - n, m), self.nh, self.nkv)
-        return out, spread, dot
+        return out, spread, dot, mass
 
     def check(self, got):
-        out, spread, dot = self.want()
+        out, *errs = self.want()
         live = slice(self.q_starts[0], self.q_starts[-1])
-        bound = so.attention_bound(out, spread, dot, self.hd, UNIT_P[self.qt], UNIT[self.qt])
+        bound = so.attention_bound(out, *errs, self.hd, UNIT_P[self.qt], UNIT[self.qt])
         err = np.abs(got - out)[live]
         assert np.all(err <= bound[live]), f"{(err / bound[live]).max():.3g} of the bound, max err {err.max():.3g}"
         assert np.all(got[:live.start] == 7.0) and np.all(got[live.stop:] == 7.0)
@@ -148,8 +148,8 @@ def test_large_scores_pick_one_key(lz, device, suite, qt, kt):
 
     c = Packed(lz, device, suite, 64, 2, 2, [140], [200], qt, kt, edit=edit)
     got = c.run()
-    out, spread, dot = c.want()
-    bound = so.attention_bound(out, spread, dot, 64, UNIT_P[qt], UNIT[qt])
+    out, *errs = c.want()
+    bound = so.attention_bound(out, *errs, 64, UNIT_P[qt], UNIT[qt])
     assert np.all(np.abs(got - out) <= bound)
 
 
