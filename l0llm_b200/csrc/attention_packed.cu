@@ -1,80 +1,581 @@
-// Causal attention over packed sequences (sm_100a): one CTA per (query row, query head), a thread per key of a tile
-// for the scores and a thread per head dimension for the values, online softmax over the tiles.
+// Causal attention over packed sequences on the 5th-generation tensor cores (sm_100a): 16-bit queries. f32 queries
+// take attention_packed_f32.cu.
+//
+// A unit of work is two tiles of 128 query rows of one sequence that read the same keys: two query heads of one KV
+// head over the same rows where the group is even (PAIR), else two consecutive row blocks of one head. CTAs (one per
+// SM) draw units from a counter, the longest of a sequence first; the kernel reads the sequences' starts on the
+// device, so one launch serves any mix of lengths. Roles of a CTA's 12 warps:
+//   0     draws units, issues the TMA loads: Q tiles, then K and V tiles of 128 rows through a ring of four stages
+//   1     issues the MMAs: S_t = Q_t K^T and O_t += P_t V, S, P and O in tensor memory (S 128 columns a tile, P over
+//         the S it came from, O HD columns), V read as it lies (N-major operand)
+//   2-3   guard the V tiles that the mask cuts (below)
+//   4-7   softmax of tile 0, a thread per row; 8-11 of tile 1
+// While one tile's softmax runs the tensor cores work on the other tile. The softmax is online in exp2 with a lazy
+// reference: O is rescaled only when a row's maximum has grown by 2^8, which after the first tiles is rare, and then
+// by the row's own softmax thread: S(j) is issued behind O += P(j - 1) V(j - 1), so whoever has S(j) may touch O.
+//
+// Rows and keys of neighbouring sequences share the tiles' edges. Scores out of a row's sight are replaced, not
+// added to, so nothing of K reaches it; but 0 * NaN is NaN in P V. So in a tile that some row sees only in part the
+// guard zeroes value rows behind the sequence, and value rows that hold an infinity or a NaN, which it notes; the
+// rows that do see such a key add its share in the epilogue.
+//
+// Probabilities are rounded once to the operands' type (its MMA takes no other), their sum is taken before that.
+//
+// Bound by the tensor cores and the exponentials alike: 2 x 128 x 128 exponentials and four 128 x 128 x HD products
+// take about 2048 cycles each at HD 128.
+#include <mutex>
+
 #include "ops.cuh"
 #include "packed.cuh"
+#include "packed_attn.cuh"
+#include "suite.h"
+#include "tma.cuh"
 
 namespace l0b {
 
 namespace {
 
-template <typename TQ, typename TK, int HD>
-__global__ void __launch_bounds__(128) attn_packed_rows_kernel(const PackedAttnParams p) {
-    __shared__ float q_s[HD], w_s[128], red[32];
-    pdl_wait();
-    pdl_launch_dependents();
-    const int t = blockIdx.x, h = blockIdx.y, kvh = h / (p.nh / p.nkv), tid = threadIdx.x;
-    const int seq = block_find_sequence(p.q_starts, p.count, t);
-    if (seq < 0) return;
-    const int first = p.q_starts[seq], end = p.q_starts[seq + 1];
-    if (t >= end) return;
-    const int k0_raw = p.kv_starts[seq], k1_raw = p.kv_starts[seq + 1];
-    const int k0 = max(0, min(k0_raw, p.kv_tokens)), m_keys = max(0, min(k1_raw, p.kv_tokens) - k0);
-    if (tid == 0 && (first < 0 || end > p.tokens || k0_raw != k0 || k1_raw != k0 + m_keys)) flag_bad_index(p.error);
-    const long long seen_raw = static_cast<long long>(m_keys) - end + t + 1;
-    const int seen = static_cast<int>(seen_raw < 0 ? 0 : seen_raw > m_keys ? m_keys : seen_raw);
-    const TQ* q = static_cast<const TQ*>(p.q) + t * p.q_stride + static_cast<long long>(h) * HD;
-    if (tid < HD) q_s[tid] = load_as_float(q, DT<TQ>::id, tid) * p.scale;
-    __syncthreads();
-    const TK* k = static_cast<const TK*>(p.k) + k0 * p.k_stride + kvh * HD;
-    const TK* v = static_cast<const TK*>(p.v) + k0 * p.v_stride + kvh * HD;
-    float m = kNegInf, l = 0.f, acc = 0.f;
-    for (int j0 = 0; j0 < seen; j0 += 128) {
-        const int j = j0 + tid;
-        float s = kNegInf;
-        if (j < seen) {
-            s = 0.f;
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                load8_f32(k + j * p.k_stride + d, x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s = fmaf(q_s[d + i], x[i], s);
-            }
-        }
-        float top = warp_max(s);
-        __syncthreads();
-        if ((tid & 31) == 0) red[tid >> 5] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float next = fmaxf(m, top), keep = m == kNegInf ? 0.f : expf(m - next);
-        const float w = j < seen ? expf(s - next) : 0.f;
-        m = next;
-        l = l * keep + block_sum(w, red);
-        w_s[tid] = w;
-        __syncthreads();
-        acc *= keep;
-        if (tid < HD) {
-            const int n = min(128, seen - j0);
-            for (int i = 0; i < n; ++i) acc += w_s[i] * load_as_float(v + (j0 + i) * p.v_stride, DT<TK>::id, tid);
-        }
-    }
-    if (tid < HD)
-        store_from_float(p.out, DT<TQ>::id, t * p.out_stride + static_cast<long long>(h) * HD + tid, seen > 0 ? acc / l : 0.f);
+constexpr int kRows = 128;     // query rows and keys of a tile
+constexpr int kRing = 4;       // K and V tiles in shared memory
+constexpr int kUnitSlots = 4;  // drawn units in flight
+constexpr int kThreads = 384;
+constexpr int kSub = kRows * 128;  // bytes of 128 rows of 64 16-bit columns, one 128-byte-swizzled block
+
+struct PackedLaunch {
+    CUtensorMap qmap, kmap, vmap;  // [rows, heads * hd], box {64, 128}
+    PackedAttnParams a;
+    unsigned* counters;  // [0] units drawn beyond each CTA's first, [1] CTAs done; zero at rest
+};
+
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D (+)= A B^T, A and B in shared memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+// D (+)= A B, A in tensor memory.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+// Operand blocks of 128-byte swizzled rows. K-major (Q, K): eight-row groups 1024 bytes apart. N-major (V): the same
+// groups along the keys, blocks of 64 columns kSub apart.
+__device__ __forceinline__ uint64_t k_major_desc(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t n_major_desc(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(kSub >> 4) << 16) | (64ull << 32) |
+           (1ull << 46) | (2ull << 61);
 }
 
-template <typename TQ, typename TK>
-l0b_status launch_as(l0b_device* d, const PackedAttnParams& p) {
-    const dim3 grid(p.tokens, p.nh);
-    if (p.hd == 64) return d->launch(attn_packed_rows_kernel<TQ, TK, 64>, grid, dim3(128), 0, p);
-    return d->launch(attn_packed_rows_kernel<TQ, TK, 128>, grid, dim3(128), 0, p);
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+// Waits for this thread's tensor-memory loads; the registers pass through, so no use of them moves above it.
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+          "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+          "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+          "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+
+// One unit, as every role works it out from its number.
+struct Unit {
+    PackedSeq s;
+    int head[2], tok[2];  // of each tile: query head, first row within the sequence
+    int rows[2], nt[2];   // live rows, key tiles
+    int full[2];          // key tiles that every row of the query tile sees whole
+    int key_tiles;        // the larger nt
+
+    __device__ __forceinline__ bool cut(int j) const {  // some row sees key tile j in part
+        return (j < nt[0] && j >= full[0]) || (j < nt[1] && j >= full[1]);
+    }
+    __device__ __forceinline__ int first_cut() const {
+        const int c0 = nt[0] ? full[0] : key_tiles, c1 = nt[1] ? full[1] : key_tiles;
+        return min(c0, c1);
+    }
+};
+
+template <bool PAIR>
+__device__ __forceinline__ int units_of(const PackedAttnParams& a, int n) {
+    return PAIR ? (n + kRows - 1) / kRows * (a.nh / 2) : (n + 2 * kRows - 1) / (2 * kRows) * a.nh;
+}
+
+template <bool PAIR>
+__device__ __forceinline__ Unit unit_at(const PackedAttnParams& a, const int* pre, int u) {
+    int lo = 0, hi = a.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= u) lo = mid;
+        else hi = mid;
+    }
+    Unit x;
+    x.s = packed_seq(a, lo);
+    const int sets = PAIR ? a.nh / 2 : a.nh, r = u - pre[lo];
+    const int blocks = (pre[lo + 1] - pre[lo]) / sets;
+    const int block = blocks - 1 - r / sets, set = r % sets;  // late rows see the most keys: first
+    x.head[0] = PAIR ? 2 * set : set;
+    x.head[1] = PAIR ? 2 * set + 1 : set;
+    x.tok[0] = block * (PAIR ? kRows : 2 * kRows);
+    x.tok[1] = PAIR ? x.tok[0] : x.tok[0] + kRows;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        x.rows[t] = max(0, min(kRows, x.s.n - x.tok[t]));
+        const int first = x.s.m - x.s.n + x.tok[t], last = first + x.rows[t] - 1;
+        x.nt[t] = x.rows[t] > 0 && last >= 0 ? last / kRows + 1 : 0;
+        x.full[t] = min(x.nt[t], max(0, first + 1) / kRows);
+    }
+    x.key_tiles = max(x.nt[0], x.nt[1]);
+    return x;
+}
+
+template <bool BF, int HD, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_constant__ PackedLaunch L) {
+    using T = typename std::conditional<BF, __nv_bfloat16, __half>::type;
+    constexpr int BLOCKS = HD / 64, TILE = BLOCKS * kSub;
+    constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(BF) << 7) | (static_cast<uint32_t>(BF) << 10) |
+                                 (static_cast<uint32_t>(kRows >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+    constexpr uint32_t kIdescO = (1u << 4) | (static_cast<uint32_t>(BF) << 7) | (static_cast<uint32_t>(BF) << 10) | (1u << 16) |
+                                 (static_cast<uint32_t>(HD >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* q_s = smem;               // [2][TILE]
+    uint8_t* kv_s = smem + 2 * TILE;   // [kRing][TILE]
+    int* pre = reinterpret_cast<int*>(kv_s + kRing * TILE);  // [count + 1] units before each sequence
+    __shared__ __align__(8) uint64_t bars[2 + 2 * kRing + 4 * 2 + kRing + 2 * kUnitSlots];
+    __shared__ int unit_s[kUnitSlots], scan_s[kThreads / 32];
+    __shared__ unsigned long long rows_s;
+    // Value rows that are not finite: [unit & 7][cut tile & 3]. The roles are at most kUnitSlots units apart.
+    __shared__ uint32_t bad_s[8][4][4];
+    __shared__ uint32_t tmem_s;
+    const PackedAttnParams& a = L.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t bar0 = smem_addr(bars);
+    const uint32_t q_full = bar0, q_empty = bar0 + 8, kv_full = bar0 + 16, kv_empty = kv_full + 8 * kRing;
+    const uint32_t s_full = kv_empty + 8 * kRing, p_ready = s_full + 16, o_full = p_ready + 16, o_empty = o_full + 16;
+    const uint32_t v_ok = o_empty + 16, drawn = v_ok + 8 * kRing, read = drawn + 8 * kUnitSlots;
+
+    if (threadIdx.x == 0) {
+        bar_init(q_full, 1);
+        bar_init(q_empty, 1);
+        for (int i = 0; i < kRing; ++i) {
+            bar_init(kv_full + 8 * i, 1);
+            bar_init(kv_empty + 8 * i, i & 1 ? 3 : 1);  // V stages: the MMAs and both guard warps
+            bar_init(v_ok + 8 * i, 2);
+        }
+        for (int t = 0; t < 2; ++t) {
+            bar_init(s_full + 8 * t, 1);
+            bar_init(p_ready + 8 * t, kRows);
+            bar_init(o_full + 8 * t, 1);
+            bar_init(o_empty + 8 * t, kRows);
+        }
+        for (int i = 0; i < kUnitSlots; ++i) {
+            bar_init(drawn + 8 * i, 1);
+            bar_init(read + 8 * i, 11);  // MMA thread, two guard warps, eight softmax warps
+        }
+        bar_init_fence();
+        rows_s = 0;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.qmap)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.kmap)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.vmap)) : "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_before();
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = tmem_s;
+
+    const bool fine = packed_scan(a, pre, scan_s, &rows_s, [&](int n) { return units_of<PAIR>(a, n); });
+    const int total = pre[a.count];
+    bool ok = true;  // false once a bounded wait gave up: the role stops
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (ok) ok = bar_wait(bar, parity);
+        return ok;
+    };
+    auto wait_warp = [&](uint32_t bar, uint32_t parity) {  // by a whole warp, which goes on or stops together
+        if (ok) ok = bar_wait(bar, parity);
+        return ok = __all_sync(0xffffffffu, ok);
+    };
+    // The next drawn unit, or -1 at the end.
+    int taken = 0;
+    auto next_unit = [&](bool whole_warp) {
+        const int slot = taken % kUnitSlots;
+        const uint32_t parity = (taken / kUnitSlots) & 1;
+        if (!(whole_warp ? wait_warp(drawn + 8 * slot, parity) : wait(drawn + 8 * slot, parity))) return -1;
+        const int u = unit_s[slot];
+        if (whole_warp) __syncwarp();
+        if (lane == 0) bar_arrive(read + 8 * slot);
+        ++taken;
+        return u;
+    };
+
+    if (!fine) {
+        // starts that name rows more than once: nothing runs
+    } else if (warp == 0) {
+        if (lane == 0) {
+            proxy_fence();
+            int e = 0, q_uses = 0;
+            int u = blockIdx.x < static_cast<unsigned>(total) ? static_cast<int>(blockIdx.x) : -1;
+            for (int i = 0; ok; ++i) {
+                const int slot = i % kUnitSlots;
+                if (!wait(read + 8 * slot, ((i / kUnitSlots) & 1) ^ 1)) break;
+                unit_s[slot] = u;
+                bar_arrive(drawn + 8 * slot);
+                if (u < 0) break;
+                const Unit x = unit_at<PAIR>(a, pre, u);
+                const unsigned ahead = atomicAdd(L.counters, 1u) + gridDim.x;
+                u = ahead < static_cast<unsigned>(total) ? static_cast<int>(ahead) : -1;
+                if (x.key_tiles == 0) continue;
+                if (!wait(q_empty, (q_uses & 1) ^ 1)) break;
+                ++q_uses;
+                bar_expect(q_full, ((x.nt[0] > 0) + (x.nt[1] > 0)) * TILE);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (x.nt[t] == 0) continue;
+#pragma unroll
+                    for (int b = 0; b < BLOCKS; ++b)
+                        tma_load(smem_addr(q_s) + t * TILE + b * kSub, &L.qmap, q_full, x.head[t] * HD + 64 * b, x.s.q0 + x.tok[t]);
+                }
+                const int kvh = x.head[0] / (a.nh / a.nkv);
+                for (int j = 0; j < x.key_tiles && ok; ++j) {
+#pragma unroll
+                    for (int w = 0; w < 2; ++w, ++e) {
+                        const int st = e % kRing;
+                        if (!wait(kv_empty + 8 * st, ((e / kRing) & 1) ^ 1)) break;
+                        bar_expect(kv_full + 8 * st, TILE);
+#pragma unroll
+                        for (int b = 0; b < BLOCKS; ++b)
+                            tma_load(smem_addr(kv_s) + st * TILE + b * kSub, w ? &L.vmap : &L.kmap, kv_full + 8 * st,
+                                     kvh * HD + 64 * b, x.s.k0 + j * kRows);
+                    }
+                }
+            }
+            if (!ok) {  // no copy of this CTA's stays in flight behind it
+                if (q_uses > 0) bar_wait(q_full, (q_uses - 1) & 1);
+                for (int i = max(0, e - kRing); i < e; ++i) bar_wait(kv_full + 8 * (i % kRing), (i / kRing) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int e = 0, q_uses = 0;
+            uint32_t p_uses[2] = {0, 0}, o_uses[2] = {0, 0}, guarded[kRing / 2] = {0, 0};  // V takes the odd stages
+            for (int u = next_unit(false); u >= 0 && ok; u = next_unit(false)) {
+                const Unit x = unit_at<PAIR>(a, pre, u);
+                if (x.key_tiles == 0) continue;
+                if (!wait(q_full, q_uses & 1)) break;
+                ++q_uses;
+                auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
+                    const int st = (e + 2 * j) % kRing;
+                    if (!wait(kv_full + 8 * st, ((e + 2 * j) / kRing) & 1)) return;
+                    tc_after();
+                    const uint32_t q = smem_addr(q_s) + t * TILE, k = smem_addr(kv_s) + st * TILE;
+#pragma unroll
+                    for (int i = 0; i < HD / 16; ++i) {
+                        const uint32_t at = (i >> 2) * kSub + (i & 3) * 32;
+                        mma_ss(tmem + t * kRows, k_major_desc(q + at), k_major_desc(k + at), kIdescS, i > 0);
+                    }
+                    tc_commit(s_full + 8 * t);
+                    if (t == (j < x.nt[1] ? 1 : 0)) {  // the last tile that reads K_j
+                        tc_commit(kv_empty + 8 * st);
+                        if (j == x.key_tiles - 1) tc_commit(q_empty);
+                    }
+                };
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    if (x.nt[t] > 0) scores(t, 0);
+                for (int j = 0; j < x.key_tiles && ok; ++j) {
+                    bool have_v = false;
+                    const int st = (e + 2 * j + 1) % kRing;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (j >= x.nt[t] || !ok) continue;
+                        if (!have_v) {
+                            if (!wait(kv_full + 8 * st, ((e + 2 * j + 1) / kRing) & 1)) break;
+                            if (x.cut(j) && !wait(v_ok + 8 * st, guarded[st >> 1]++ & 1)) break;
+                            have_v = true;
+                        }
+                        if (j == 0 && !wait(o_empty + 8 * t, (o_uses[t]++ & 1) ^ 1)) break;
+                        if (!wait(p_ready + 8 * t, p_uses[t]++ & 1)) break;
+                        tc_after();
+                        const uint32_t v = smem_addr(kv_s) + st * TILE;
+#pragma unroll
+                        for (int i = 0; i < kRows / 16; ++i)
+                            mma_ts(tmem + 2 * kRows + t * HD, tmem + t * kRows + i * 8, n_major_desc(v + i * 2048), kIdescO,
+                                   j > 0 || i > 0);
+                        if (t == (j < x.nt[1] ? 1 : 0)) tc_commit(kv_empty + 8 * st);
+                        if (j + 1 < x.nt[t]) scores(t, j + 1);
+                        else tc_commit(o_full + 8 * t);
+                    }
+                }
+                e += 2 * x.key_tiles;
+            }
+            if (!ok) {
+                tc_commit(q_empty);  // MMAs in flight end before the tensor memory goes
+                bar_wait(q_empty, (q_uses - 1) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        int e = 0;
+        for (int i = 0;; ++i) {
+            const int u = next_unit(true);
+            if (u < 0 || !ok) break;
+            const Unit x = unit_at<PAIR>(a, pre, u);
+            int nth = 0;
+            for (int j = 0; j < x.key_tiles && ok; ++j) {
+                // Every V tile is waited for, so that the guard is never a round of the ring ahead or behind.
+                const int st = (e + 2 * j + 1) % kRing;
+                if (!wait_warp(kv_full + 8 * st, ((e + 2 * j + 1) / kRing) & 1)) break;
+                if (!x.cut(j)) {
+                    if (lane == 0) bar_arrive(kv_empty + 8 * st);
+                    continue;
+                }
+                uint8_t* v = kv_s + st * TILE;
+                constexpr int LANES = BLOCKS * 8, AT_ONCE = 32 / LANES;  // lanes a row, rows at once
+                const int live = x.s.m - j * kRows, sub = lane / LANES, c = lane % LANES;
+                uint32_t bad[2] = {0, 0};
+#pragma unroll
+                for (int r0 = 0; r0 < 64; r0 += AT_ONCE) {
+                    const int r = (warp - 2) * 64 + r0 + sub;
+                    uint4* at = reinterpret_cast<uint4*>(v + (c >> 3) * kSub + r * 128 + (c & 7) * 16);
+                    const uint4 w = *at;
+                    const bool odd = not_finite<BF>(w.x) || not_finite<BF>(w.y) || not_finite<BF>(w.z) || not_finite<BF>(w.w);
+                    const uint32_t hit = __ballot_sync(0xffffffffu, odd && r < live);
+                    const uint32_t mine = (hit >> (sub * LANES)) & ((1u << LANES) - 1u);
+                    if (mine || r >= live) *at = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < AT_ONCE; ++k)
+                        if ((hit >> (k * LANES)) & ((1u << LANES) - 1u)) bad[(r0 + k) >> 5] |= 1u << ((r0 + k) & 31);
+                }
+                if (lane < 2) bad_s[i & 7][nth & 3][(warp - 2) * 2 + lane] = lane ? bad[1] : bad[0];
+                ++nth;
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) {
+                    bar_arrive(v_ok + 8 * st);
+                    bar_arrive(kv_empty + 8 * st);
+                }
+            }
+            e += 2 * x.key_tiles;
+        }
+    } else {
+        const int t = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + t * kRows + lanes, o_at = tmem + 2 * kRows + t * HD + lanes;
+        const float c = a.scale * 1.44269504088896341f;
+        uint32_t s_uses = 0, o_uses = 0;
+        for (int i = 0;; ++i) {
+            const int u = next_unit(true);
+            if (u < 0 || !ok) break;
+            const Unit x = unit_at<PAIR>(a, pre, u);
+            const int nt = x.nt[t], limit = x.s.m - x.s.n + x.tok[t] + row;  // the last key this row sees
+            float ref = kNegInf, sum = 0.f;  // weights are exp2((s - ref) c)
+            for (int j = 0; j < nt; ++j) {
+                if (!wait_warp(s_full + 8 * t, s_uses++ & 1)) break;
+                tc_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) tmem_load32(s_at + 32 * b, s[b]);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) tmem_loaded(s[b]);
+                if (j >= x.full[t]) {
+                    const int last = limit - j * kRows;
+#pragma unroll
+                    for (int k = 0; k < 128; ++k)
+                        if (k > last) s[k >> 5][k & 31] = __float_as_uint(kNegInf);
+                }
+                float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) top[b] = fmaxf(top[b], __uint_as_float(s[b][k]));
+                }
+                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                // The reference moves when it must: at the first keys seen, or when weights would pass 2^8.
+                const bool move = most > ref && !((most - ref) * c <= 8.f);
+                if (__any_sync(0xffffffffu, move)) {
+                    const float by = move ? exp2_fast((ref - most) * c) : 1.f;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int b = 0; b < HD / 32; ++b) {
+                            uint32_t o[32];
+                            tmem_load32(o_at + 32 * b, o);
+                            tmem_loaded(o);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+                            tmem_store32(o_at + 32 * b, o);
+                        }
+                    }
+                    if (move) {
+                        ref = most;
+                        sum *= by;
+                    }
+                }
+                __syncwarp();
+                const float shift = ref == kNegInf ? 0.f : ref * c;
+                const float2 c2 = make_float2(c, c), shift2 = make_float2(-shift, -shift);
+                float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        float2 y = ffma2(make_float2(__uint_as_float(s[b][2 * k]), __uint_as_float(s[b][2 * k + 1])), c2, shift2);
+                        y.x = exp2_fast(y.x);
+                        y.y = exp2_fast(y.y);
+                        add[k & 1] = fadd2(add[k & 1], y);
+                        w[k] = pack2<T>(y.x, y.y);
+                    }
+                    tmem_store16(s_at + 16 * b, w);
+                }
+                sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_before();
+                bar_arrive(p_ready + 8 * t);
+            }
+            if (x.rows[t] == 0 || !ok) continue;
+            if (nt > 0) {
+                if (!wait_warp(o_full + 8 * t, o_uses++ & 1)) break;
+                tc_after();
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T* out = static_cast<T*>(a.out) + static_cast<long long>(x.s.q0 + x.tok[t] + row) * a.out_stride + x.head[t] * HD;
+#pragma unroll 1
+            for (int b = 0; b < HD / 32; ++b) {
+                uint32_t o[32];
+                if (nt > 0) {
+                    tmem_load32(o_at + 32 * b, o);
+                    tmem_loaded(o);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = 0;
+                }
+                if (b == HD / 32 - 1 && nt > 0) {
+                    tc_before();
+                    bar_arrive(o_empty + 8 * t);
+                }
+                if (row < x.rows[t]) {
+                    // Values that the guard set aside, where this row sees them.
+                    int nth = 0;
+                    for (int j = x.first_cut(); j < x.key_tiles; ++j) {
+                        if (!x.cut(j)) continue;
+                        for (int w = 0; w < 4; ++w) {
+                            for (uint32_t bits = bad_s[i & 7][nth & 3][w]; bits; bits &= bits - 1) {
+                                const int key = j * kRows + w * 32 + __ffs(bits) - 1;
+                                if (key > limit) break;
+                                add_value_share<T, HD>(a, x.s, x.head[t], x.tok[t] + row, key, c, ref == kNegInf ? 0.f : ref * c, b, o);
+                            }
+                        }
+                        ++nth;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        uint4 w;
+                        w.x = pack2<T>(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
+                        w.y = pack2<T>(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
+                        w.z = pack2<T>(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
+                        w.w = pack2<T>(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
+                        *reinterpret_cast<uint4*>(out + 32 * b + k) = w;
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    if (!ok && a.error) atomicOr(a.error, 1);
+    tc_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    if (threadIdx.x == 0 && fine) {
+        __threadfence();
+        if (atomicAdd(L.counters + 1, 1u) == gridDim.x - 1) {  // every CTA has drawn its last
+            L.counters[0] = 0;
+            L.counters[1] = 0;
+        }
+    }
+}
+
+template <bool BF, int HD, bool PAIR>
+l0b_status launch_tc(l0b_suite* s, l0b_device* d, const PackedAttnParams& a) {
+    auto kernel = packed_tc_kernel<BF, HD, PAIR>;
+    constexpr size_t tiles = 1024 + static_cast<size_t>(2 + kRing) * (HD / 64) * kSub;
+    {
+        static bool configured[64] = {};
+        static std::mutex mu;
+        std::lock_guard<std::mutex> lock(mu);
+        if (d->index >= 64 || !configured[d->index]) {
+            L0B_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                static_cast<int>(tiles + 4 * (kMaxSequences + 1))));
+            if (d->index < 64) configured[d->index] = true;
+        }
+    }
+    PackedLaunch L;
+    std::memset(&L, 0, sizeof L);
+    const auto type = BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const long long kvw = static_cast<long long>(a.nkv) * HD, kv_rows = a.kv_tokens > 0 ? a.kv_tokens : 1;
+    L0B_TRY(tensor_map_2d(&L.qmap, type, 2, a.q, static_cast<long long>(a.nh) * HD, a.tokens, a.q_stride, 64, kRows,
+                          CU_TENSOR_MAP_SWIZZLE_128B));
+    L0B_TRY(tensor_map_2d(&L.kmap, type, 2, a.k, kvw, kv_rows, a.k_stride, 64, kRows, CU_TENSOR_MAP_SWIZZLE_128B));
+    L0B_TRY(tensor_map_2d(&L.vmap, type, 2, a.v, kvw, kv_rows, a.v_stride, 64, kRows, CU_TENSOR_MAP_SWIZZLE_128B));
+    L.a = a;
+    L.counters = s->packed_counters;
+    return d->launch(kernel, dim3(d->sm_count), dim3(kThreads), tiles + 4 * (static_cast<size_t>(a.count) + 1), L);
+}
+
+template <bool BF>
+l0b_status launch_as(l0b_suite* s, l0b_device* d, const PackedAttnParams& a) {
+    const bool pair = (a.nh / a.nkv) % 2 == 0;
+    if (a.hd == 64) return pair ? launch_tc<BF, 64, true>(s, d, a) : launch_tc<BF, 64, false>(s, d, a);
+    return pair ? launch_tc<BF, 128, true>(s, d, a) : launch_tc<BF, 128, false>(s, d, a);
 }
 
 }  // namespace
 
-l0b_status k_attention_packed(l0b_suite*, l0b_device* d, const PackedAttnParams& p) {
-    L0B_REQUIRE(p.nh <= 65535, L0B_ERR_OUT_OF_RANGE, "heads %d exceed 65535", p.nh);
-    if (p.kv_dtype == L0B_F16)
-        return p.q_dtype == L0B_F32 ? launch_as<float, __half>(d, p) : launch_as<__half, __half>(d, p);
-    return p.q_dtype == L0B_F32 ? launch_as<float, __nv_bfloat16>(d, p) : launch_as<__nv_bfloat16, __nv_bfloat16>(d, p);
+l0b_status k_attention_packed(l0b_suite* s, l0b_device* d, const PackedAttnParams& p) {
+    if (p.q_dtype == L0B_F32) return k_attention_packed_f32(s, d, p);
+    // Units are counted in 32 bits: blocks of rows times heads.
+    L0B_REQUIRE((static_cast<long long>(p.tokens) / kRows + p.count) * p.nh <= INT32_MAX, L0B_ERR_OUT_OF_RANGE,
+                "%d rows of %d heads are too many for one call", p.tokens, p.nh);
+    return p.kv_dtype == L0B_BF16 ? launch_as<true>(s, d, p) : launch_as<false>(s, d, p);
 }
 
 }  // namespace l0b

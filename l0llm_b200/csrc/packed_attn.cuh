@@ -1,0 +1,94 @@
+// Shared by the packed-attention kernels (attention_packed.cu, attention_packed_f32.cu): the sequences' extents, the
+// scan over them, and the values that a cut tile's guard sets aside.
+#pragma once
+
+#include "ops.cuh"
+#include "packed.cuh"
+
+namespace l0b {
+
+l0b_status k_attention_packed_f32(l0b_suite* s, l0b_device* d, const PackedAttnParams& p);
+
+// Rows of one sequence, kept inside the buffers whatever its starts say.
+struct PackedSeq {
+    int q0, n;  // first query row, query rows
+    int k0, m;  // first key row, key rows
+};
+
+__device__ __forceinline__ PackedSeq packed_seq(const PackedAttnParams& a, int i) {
+    PackedSeq s;
+    s.q0 = max(__ldg(a.q_starts + i), 0);
+    s.n = max(0, min(__ldg(a.q_starts + i + 1), a.tokens) - s.q0);
+    s.k0 = max(0, min(__ldg(a.kv_starts + i), a.kv_tokens));
+    s.m = max(0, min(__ldg(a.kv_starts + i + 1), a.kv_tokens) - s.k0);
+    return s;
+}
+
+// pre[i] = the sum of units(n) over the sequences before i, pre[count] the total, by the whole CTA. False (and the
+// error flag) when the sequences together have more rows than the buffer, which ascending starts never have.
+template <typename F>
+__device__ __forceinline__ bool packed_scan(const PackedAttnParams& a, int* pre, int* warp_sums, unsigned long long* rows_s,
+                                            F units) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int per = (a.count + blockDim.x - 1) / blockDim.x, i0 = threadIdx.x * per, i1 = min(a.count, i0 + per);
+    int mine = 0;
+    long long rows = 0;
+    bool bad = false;
+    for (int i = i0; i < i1; ++i) {
+        const PackedSeq s = packed_seq(a, i);
+        mine += units(s.n);
+        rows += s.n;
+        bad |= __ldg(a.q_starts + i) < 0 || __ldg(a.q_starts + i + 1) > a.tokens || __ldg(a.kv_starts + i) < 0 ||
+               __ldg(a.kv_starts + i + 1) > a.kv_tokens || __ldg(a.q_starts + i) > __ldg(a.q_starts + i + 1) ||
+               __ldg(a.kv_starts + i) > __ldg(a.kv_starts + i + 1);
+    }
+    if (bad && blockIdx.x == 0) flag_bad_index(a.error);
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+    }
+    if (lane == 31) warp_sums[warp] = sum;
+    if (rows) atomicAdd(rows_s, static_cast<unsigned long long>(rows));
+    __syncthreads();
+    const bool fine = *rows_s <= static_cast<unsigned long long>(a.tokens);
+    if (!fine && threadIdx.x == 0) flag_bad_index(a.error);
+    int before = sum - mine;
+    for (int w = 0; w < warp; ++w) before += warp_sums[w];
+    for (int i = i0; i < i1; ++i) {
+        pre[i] = before;
+        before += units(packed_seq(a, i).n);
+    }
+    if (threadIdx.x == 0) {
+        int all = 0;
+        for (int w = 0; w < warps; ++w) all += warp_sums[w];
+        pre[a.count] = all;
+    }
+    __syncthreads();
+    return fine;
+}
+
+// Whether one of a pair of 16-bit values is an infinity or a NaN (every exponent bit set).
+template <bool BF>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+    const uint32_t e = BF ? 0x7F80u : 0x7C00u;
+    return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+// o[0, 32) (f32 bits) += weight * value of one key, dims 32 b .. 32 b + 31, the weight worked out anew: for the few
+// values that are not finite in tiles that the mask cuts.
+template <typename T, int HD>
+__device__ __noinline__ void add_value_share(const PackedAttnParams& a, const PackedSeq& s, int head, int row, int key, float c,
+                                             float shift, int b, uint32_t (&o)[32]) {
+    const int kvh = head / (a.nh / a.nkv);
+    const T* k = static_cast<const T*>(a.k) + static_cast<long long>(s.k0 + key) * a.k_stride + kvh * HD;
+    const T* v = static_cast<const T*>(a.v) + static_cast<long long>(s.k0 + key) * a.v_stride + kvh * HD + 32 * b;
+    const long long q = static_cast<long long>(s.q0 + row) * a.q_stride + static_cast<long long>(head) * HD;
+    float dot = 0.f;
+    for (int d = 0; d < HD; ++d) dot = fmaf(load_as_float(a.q, a.q_dtype, q + d), load_as_float(k, DT<T>::id, d), dot);
+    const float w = exp2f(dot * c - shift);
+    for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(fmaf(w, load_as_float(v, DT<T>::id, d), __uint_as_float(o[d])));
+}
+
+}  // namespace l0b

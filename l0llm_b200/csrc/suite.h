@@ -39,6 +39,7 @@ struct l0b_suite {
     // arrival counter per team, zero at rest. Launches of one stream take turns, so all share them.
     float* q8_part = nullptr;
     unsigned* q8_counters = nullptr;
+    unsigned* packed_counters = nullptr;  // packed attention: units drawn, CTAs done; zero at rest
     std::map<std::pair<int, double>, float*> rope_tables;
     ~l0b_suite();
 };
