@@ -244,8 +244,11 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         return u;
     };
 
+    // The launch's 168 registers a thread are dealt anew: 72 for the first warpgroup, 216 for the softmax threads.
+    // Starts that name rows more than once: nothing runs.
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (!fine) {
-        // starts that name rows more than once: nothing runs
     } else if (warp == 0) {
         if (lane == 0) {
             proxy_fence();
@@ -351,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
             }
         }
         __syncwarp();
-    } else if (warp < 4) {
+    } else {
         int e = 0;
         for (int i = 0;; ++i) {
             const int u = next_unit(true);
@@ -394,7 +397,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
             }
             e += 2 * x.key_tiles;
         }
+    }
     } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (fine) {
         const int t = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + t * kRows + lanes, o_at = tmem + 2 * kRows + t * HD + lanes;
@@ -422,9 +428,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                 }
                 float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
+                for (int k = 0; k < 32; k += 2) {
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) top[b] = fmaxf(top[b], __uint_as_float(s[b][k]));
+                    for (int b = 0; b < 4; ++b)
+                        top[b] = fmaxf(fmaxf(top[b], __uint_as_float(s[b][k])), __uint_as_float(s[b][k + 1]));
                 }
                 const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 // The reference moves when it must: at the first keys seen, or when weights would pass 2^8.
@@ -517,6 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                 __syncwarp();
             }
         }
+    }
     }
     if (!ok && a.error) atomicOr(a.error, 1);
     tc_before();
