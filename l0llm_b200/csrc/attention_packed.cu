@@ -49,20 +49,27 @@ struct PackedLaunch {
 
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+// The MMA warp runs its loop whole and elects the issuing thread in each of these: in a branch of one thread the
+// compiler moved every operand to a uniform register per MMA, and eight MMAs took 820 cycles to issue, not 512.
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+        : "memory");
 }
 // D (+)= A B^T, A and B in shared memory.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
 // D (+)= A B, A in tensor memory.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
@@ -179,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     __shared__ uint32_t bad_s[8][4][4];
     __shared__ uint32_t tmem_s;
     const PackedAttnParams& a = L.a;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t bar0 = smem_addr(bars);
     const uint32_t q_full = bar0, q_empty = bar0 + 8, kv_full = bar0 + 16, kv_empty = kv_full + 8 * kRing;
     const uint32_t s_full = kv_empty + 8 * kRing, p_ready = s_full + 16, o_full = p_ready + 16, o_empty = o_full + 16;
@@ -233,12 +240,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     };
     // The next drawn unit, or -1 at the end.
     int taken = 0;
-    auto next_unit = [&](bool whole_warp) {
+    auto next_unit = [&]() {
         const int slot = taken % kUnitSlots;
-        const uint32_t parity = (taken / kUnitSlots) & 1;
-        if (!(whole_warp ? wait_warp(drawn + 8 * slot, parity) : wait(drawn + 8 * slot, parity))) return -1;
-        const int u = unit_s[slot];
-        if (whole_warp) __syncwarp();
+        if (!wait_warp(drawn + 8 * slot, (taken / kUnitSlots) & 1)) return -1;
+        const int u = __shfl_sync(0xffffffffu, unit_s[slot], 0);
         if (lane == 0) bar_arrive(read + 8 * slot);
         ++taken;
         return u;
@@ -295,69 +300,66 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            int e = 0, q_uses = 0;
-            uint32_t p_uses[2] = {0, 0}, o_uses[2] = {0, 0}, guarded[kRing / 2] = {0, 0};  // V takes the odd stages
-            for (int u = next_unit(false); u >= 0 && ok; u = next_unit(false)) {
-                const Unit x = unit_at<PAIR>(a, pre, u);
-                if (x.key_tiles == 0) continue;
-                if (!wait(q_full, q_uses & 1)) break;
-                ++q_uses;
-                auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
-                    const int st = (e + 2 * j) % kRing;
-                    if (!wait(kv_full + 8 * st, ((e + 2 * j) / kRing) & 1)) return;
-                    tc_after();
-                    const uint32_t q = smem_addr(q_s) + t * TILE, k = smem_addr(kv_s) + st * TILE;
+        int e = 0, q_uses = 0;
+        uint32_t p_uses[2] = {0, 0}, o_uses[2] = {0, 0}, guarded[kRing / 2] = {0, 0};  // V takes the odd stages
+        for (int u = next_unit(); u >= 0 && ok; u = next_unit()) {
+            const Unit x = unit_at<PAIR>(a, pre, u);
+            if (x.key_tiles == 0) continue;
+            if (!wait_warp(q_full, q_uses & 1)) break;
+            ++q_uses;
+            auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
+                const int st = (e + 2 * j) % kRing;
+                if (!wait_warp(kv_full + 8 * st, ((e + 2 * j) / kRing) & 1)) return;
+                tc_after();
+                const uint32_t q = smem_addr(q_s) + t * TILE, k = smem_addr(kv_s) + st * TILE;
 #pragma unroll
-                    for (int i = 0; i < HD / 16; ++i) {
-                        const uint32_t at = (i >> 2) * kSub + (i & 3) * 32;
-                        mma_ss(tmem + t * kRows, k_major_desc(q + at), k_major_desc(k + at), kIdescS, i > 0);
-                    }
-                    tc_commit(s_full + 8 * t);
-                    if (t == (j < x.nt[1] ? 1 : 0)) {  // the last tile that reads K_j
-                        tc_commit(kv_empty + 8 * st);
-                        if (j == x.key_tiles - 1) tc_commit(q_empty);
-                    }
-                };
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-                    if (x.nt[t] > 0) scores(t, 0);
-                for (int j = 0; j < x.key_tiles && ok; ++j) {
-                    bool have_v = false;
-                    const int st = (e + 2 * j + 1) % kRing;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (j >= x.nt[t] || !ok) continue;
-                        if (!have_v) {
-                            if (!wait(kv_full + 8 * st, ((e + 2 * j + 1) / kRing) & 1)) break;
-                            if (x.cut(j) && !wait(v_ok + 8 * st, guarded[st >> 1]++ & 1)) break;
-                            have_v = true;
-                        }
-                        if (j == 0 && !wait(o_empty + 8 * t, (o_uses[t]++ & 1) ^ 1)) break;
-                        if (!wait(p_ready + 8 * t, p_uses[t]++ & 1)) break;
-                        tc_after();
-                        const uint32_t v = smem_addr(kv_s) + st * TILE;
-#pragma unroll
-                        for (int i = 0; i < kRows / 16; ++i)
-                            mma_ts(tmem + 2 * kRows + t * HD, tmem + t * kRows + i * 8, n_major_desc(v + i * 2048), kIdescO,
-                                   j > 0 || i > 0);
-                        if (t == (j < x.nt[1] ? 1 : 0)) tc_commit(kv_empty + 8 * st);
-                        if (j + 1 < x.nt[t]) scores(t, j + 1);
-                        else tc_commit(o_full + 8 * t);
-                    }
+                for (int i = 0; i < HD / 16; ++i) {
+                    const uint32_t at = (i >> 2) * kSub + (i & 3) * 32;
+                    mma_ss(tmem + t * kRows, k_major_desc(q + at), k_major_desc(k + at), kIdescS, i > 0);
                 }
-                e += 2 * x.key_tiles;
+                tc_commit(s_full + 8 * t);
+                if (t == (j < x.nt[1] ? 1 : 0)) {  // the last tile that reads K_j
+                    tc_commit(kv_empty + 8 * st);
+                    if (j == x.key_tiles - 1) tc_commit(q_empty);
+                }
+            };
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (x.nt[t] > 0) scores(t, 0);
+            for (int j = 0; j < x.key_tiles && ok; ++j) {
+                bool have_v = false;
+                const int st = (e + 2 * j + 1) % kRing;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (j >= x.nt[t] || !ok) continue;
+                    if (!have_v) {
+                        if (!wait_warp(kv_full + 8 * st, ((e + 2 * j + 1) / kRing) & 1)) break;
+                        if (x.cut(j) && !wait_warp(v_ok + 8 * st, guarded[st >> 1]++ & 1)) break;
+                        have_v = true;
+                    }
+                    if (j == 0 && !wait_warp(o_empty + 8 * t, (o_uses[t]++ & 1) ^ 1)) break;
+                    if (!wait_warp(p_ready + 8 * t, p_uses[t]++ & 1)) break;
+                    tc_after();
+                    const uint32_t v = smem_addr(kv_s) + st * TILE;
+#pragma unroll
+                    for (int i = 0; i < kRows / 16; ++i)
+                        mma_ts(tmem + 2 * kRows + t * HD, tmem + t * kRows + i * 8, n_major_desc(v + i * 2048), kIdescO,
+                               j > 0 || i > 0);
+                    if (t == (j < x.nt[1] ? 1 : 0)) tc_commit(kv_empty + 8 * st);
+                    if (j + 1 < x.nt[t]) scores(t, j + 1);
+                    else tc_commit(o_full + 8 * t);
+                }
             }
-            if (!ok) {
-                tc_commit(q_empty);  // MMAs in flight end before the tensor memory goes
-                bar_wait(q_empty, (q_uses - 1) & 1);
-            }
+            e += 2 * __shfl_sync(0xffffffffu, x.key_tiles, 0);  // known to be uniform, and the stages with it
         }
-        __syncwarp();
+        if (!ok) {
+            tc_commit(q_empty);  // MMAs in flight end before the tensor memory goes
+            bar_wait(q_empty, (q_uses - 1) & 1);
+        }
     } else {
         int e = 0;
         for (int i = 0;; ++i) {
-            const int u = next_unit(true);
+            const int u = next_unit();
             if (u < 0 || !ok) break;
             const Unit x = unit_at<PAIR>(a, pre, u);
             int nth = 0;
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         const float c = a.scale * 1.44269504088896341f;
         uint32_t s_uses = 0, o_uses = 0;
         for (int i = 0;; ++i) {
-            const int u = next_unit(true);
+            const int u = next_unit();
             if (u < 0 || !ok) break;
             const Unit x = unit_at<PAIR>(a, pre, u);
             const int nt = x.nt[t], limit = x.s.m - x.s.n + x.tok[t] + row;  // the last key this row sees
