@@ -116,13 +116,13 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[
 }
 
 
-// One unit, as every role works it out from its number.
+// One unit, worked out by the drawing thread and handed on in shared memory.
 struct Unit {
     PackedSeq s;
     int head[2], tok[2];  // of each tile: query head, first row within the sequence
     int rows[2], nt[2];   // live rows, key tiles
     int full[2];          // key tiles that every row of the query tile sees whole
-    int key_tiles;        // the larger nt
+    int key_tiles;        // the larger nt, -1: no more units
 
     __device__ __forceinline__ bool cut(int j) const {  // some row sees key tile j in part
         return (j < nt[0] && j >= full[0]) || (j < nt[1] && j >= full[1]);
@@ -180,10 +180,12 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     uint8_t* kv_s = smem + 2 * TILE;   // [kRing][TILE]
     int* pre = reinterpret_cast<int*>(kv_s + kRing * TILE);  // [count + 1] units before each sequence
     __shared__ __align__(8) uint64_t bars[2 + 2 * kRing + 4 * 2 + kRing + 2 * kUnitSlots];
-    __shared__ int unit_s[kUnitSlots], scan_s[kThreads / 32];
+    __shared__ Unit unit_s[kUnitSlots];
+    __shared__ int scan_s[kThreads / 32];
     __shared__ unsigned long long rows_s;
     // Value rows that are not finite: [unit & 7][cut tile & 3]. The roles are at most kUnitSlots units apart.
     __shared__ uint32_t bad_s[8][4][4];
+    __shared__ int any_bad_s[8];
     __shared__ uint32_t tmem_s;
     const PackedAttnParams& a = L.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -238,21 +240,22 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         if (ok) ok = bar_wait(bar, parity);
         return ok = __all_sync(0xffffffffu, ok);
     };
-    // The next drawn unit, or -1 at the end.
+    // The next drawn unit; false at the end.
     int taken = 0;
-    auto next_unit = [&]() {
+    auto next_unit = [&](Unit& x) {
         const int slot = taken % kUnitSlots;
-        if (!wait_warp(drawn + 8 * slot, (taken / kUnitSlots) & 1)) return -1;
-        const int u = __shfl_sync(0xffffffffu, unit_s[slot], 0);
+        if (!wait_warp(drawn + 8 * slot, (taken / kUnitSlots) & 1)) return false;
+        x = unit_s[slot];
+        __syncwarp();
         if (lane == 0) bar_arrive(read + 8 * slot);
         ++taken;
-        return u;
+        return __shfl_sync(0xffffffffu, x.key_tiles, 0) >= 0;
     };
 
-    // The launch's 168 registers a thread are dealt anew: 72 for the first warpgroup, 216 for the softmax threads.
+    // The launch's 168 registers a thread are dealt anew: 88 for the first warpgroup, 208 for the softmax threads.
     // Starts that name rows more than once: nothing runs.
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (!fine) {
     } else if (warp == 0) {
         if (lane == 0) {
@@ -262,34 +265,37 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
             for (int i = 0; ok; ++i) {
                 const int slot = i % kUnitSlots;
                 if (!wait(read + 8 * slot, ((i / kUnitSlots) & 1) ^ 1)) break;
-                unit_s[slot] = u;
-                bar_arrive(drawn + 8 * slot);
-                if (u < 0) break;
+                if (u < 0) {
+                    unit_s[slot].key_tiles = -1;
+                    bar_arrive(drawn + 8 * slot);
+                    break;
+                }
                 const Unit x = unit_at<PAIR>(a, pre, u);
+                unit_s[slot] = x;
+                any_bad_s[i & 7] = 0;
+                bar_arrive(drawn + 8 * slot);
                 const unsigned ahead = atomicAdd(L.counters, 1u) + gridDim.x;
                 u = ahead < static_cast<unsigned>(total) ? static_cast<int>(ahead) : -1;
                 if (x.key_tiles == 0) continue;
-                if (!wait(q_empty, (q_uses & 1) ^ 1)) break;
-                ++q_uses;
-                bar_expect(q_full, ((x.nt[0] > 0) + (x.nt[1] > 0)) * TILE);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (x.nt[t] == 0) continue;
+                const int kvh = x.head[0] / (a.nh / a.nkv);
+                for (int k = 0; k < 2 * x.key_tiles; ++k, ++e) {  // K_0, Q, V_0, K_1, V_1, ...
+                    const int st = e % kRing;
+                    if (!wait(kv_empty + 8 * st, ((e / kRing) & 1) ^ 1)) break;
+                    bar_expect(kv_full + 8 * st, TILE);
 #pragma unroll
                     for (int b = 0; b < BLOCKS; ++b)
-                        tma_load(smem_addr(q_s) + t * TILE + b * kSub, &L.qmap, q_full, x.head[t] * HD + 64 * b, x.s.q0 + x.tok[t]);
-                }
-                const int kvh = x.head[0] / (a.nh / a.nkv);
-                for (int j = 0; j < x.key_tiles && ok; ++j) {
+                        tma_load(smem_addr(kv_s) + st * TILE + b * kSub, k & 1 ? &L.vmap : &L.kmap, kv_full + 8 * st,
+                                 kvh * HD + 64 * b, x.s.k0 + (k >> 1) * kRows);
+                    if (k > 0) continue;
+                    if (!wait(q_empty, (q_uses & 1) ^ 1)) break;
+                    ++q_uses;
+                    bar_expect(q_full, ((x.nt[0] > 0) + (x.nt[1] > 0)) * TILE);
 #pragma unroll
-                    for (int w = 0; w < 2; ++w, ++e) {
-                        const int st = e % kRing;
-                        if (!wait(kv_empty + 8 * st, ((e / kRing) & 1) ^ 1)) break;
-                        bar_expect(kv_full + 8 * st, TILE);
+                    for (int t = 0; t < 2; ++t) {
+                        if (x.nt[t] == 0) continue;
 #pragma unroll
                         for (int b = 0; b < BLOCKS; ++b)
-                            tma_load(smem_addr(kv_s) + st * TILE + b * kSub, w ? &L.vmap : &L.kmap, kv_full + 8 * st,
-                                     kvh * HD + 64 * b, x.s.k0 + j * kRows);
+                            tma_load(smem_addr(q_s) + t * TILE + b * kSub, &L.qmap, q_full, x.head[t] * HD + 64 * b, x.s.q0 + x.tok[t]);
                     }
                 }
             }
@@ -302,8 +308,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     } else if (warp == 1) {
         int e = 0, q_uses = 0;
         uint32_t p_uses[2] = {0, 0}, o_uses[2] = {0, 0}, guarded[kRing / 2] = {0, 0};  // V takes the odd stages
-        for (int u = next_unit(); u >= 0 && ok; u = next_unit()) {
-            const Unit x = unit_at<PAIR>(a, pre, u);
+        Unit x;
+        while (next_unit(x)) {
             if (x.key_tiles == 0) continue;
             if (!wait_warp(q_full, q_uses & 1)) break;
             ++q_uses;
@@ -359,9 +365,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     } else {
         int e = 0;
         for (int i = 0;; ++i) {
-            const int u = next_unit();
-            if (u < 0 || !ok) break;
-            const Unit x = unit_at<PAIR>(a, pre, u);
+            Unit x;
+            if (!next_unit(x)) break;
             int nth = 0;
             for (int j = 0; j < x.key_tiles && ok; ++j) {
                 // Every V tile is waited for, so that the guard is never a round of the ring ahead or behind.
@@ -372,23 +377,36 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                     continue;
                 }
                 uint8_t* v = kv_s + st * TILE;
-                constexpr int LANES = BLOCKS * 8, AT_ONCE = 32 / LANES;  // lanes a row, rows at once
-                const int live = x.s.m - j * kRows, sub = lane / LANES, c = lane % LANES;
+                // A row takes LANES lanes of 16 bytes; a warp looks at AT_ONCE rows a step, eight steps in flight.
+                constexpr int LANES = BLOCKS * 8, AT_ONCE = 32 / LANES;
+                const int live = x.s.m - j * kRows, sub = lane / LANES, c = lane % LANES, base = (warp - 2) * 64;
                 uint32_t bad[2] = {0, 0};
+#pragma unroll 1
+                for (int r0 = 0; r0 < 64; r0 += 8 * AT_ONCE) {
+                    uint8_t* at = v + (c >> 3) * kSub + (base + r0 + sub) * 128 + (c & 7) * 16;
+                    uint32_t odd = 0;
 #pragma unroll
-                for (int r0 = 0; r0 < 64; r0 += AT_ONCE) {
-                    const int r = (warp - 2) * 64 + r0 + sub;
-                    uint4* at = reinterpret_cast<uint4*>(v + (c >> 3) * kSub + r * 128 + (c & 7) * 16);
-                    const uint4 w = *at;
-                    const bool odd = not_finite<BF>(w.x) || not_finite<BF>(w.y) || not_finite<BF>(w.z) || not_finite<BF>(w.w);
-                    const uint32_t hit = __ballot_sync(0xffffffffu, odd && r < live);
-                    const uint32_t mine = (hit >> (sub * LANES)) & ((1u << LANES) - 1u);
-                    if (mine || r >= live) *at = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int k = 0; k < AT_ONCE; ++k)
-                        if ((hit >> (k * LANES)) & ((1u << LANES) - 1u)) bad[(r0 + k) >> 5] |= 1u << ((r0 + k) & 31);
+                    for (int k = 0; k < 8; ++k) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(at + k * AT_ONCE * 128);
+                        odd |= static_cast<uint32_t>(not_finite<BF>(w) && base + r0 + k * AT_ONCE + sub < live) << k;
+                    }
+                    if (!__any_sync(0xffffffffu, odd != 0) && base + r0 + 8 * AT_ONCE <= live) continue;
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t hit = __ballot_sync(0xffffffffu, (odd >> k) & 1);
+                        const uint32_t row_mask = (1u << LANES) - 1u;
+                        if (((hit >> (sub * LANES)) & row_mask) || base + r0 + k * AT_ONCE + sub >= live)
+                            *reinterpret_cast<uint4*>(at + k * AT_ONCE * 128) = make_uint4(0, 0, 0, 0);
+                        for (int q = 0; q < AT_ONCE; ++q) {
+                            const int r = r0 + k * AT_ONCE + q;
+                            if ((hit >> (q * LANES)) & row_mask) bad[r >> 5] |= 1u << (r & 31);
+                        }
+                    }
                 }
-                if (lane < 2) bad_s[i & 7][nth & 3][(warp - 2) * 2 + lane] = lane ? bad[1] : bad[0];
+                if (lane < 2) {
+                    const uint32_t mine = lane ? bad[1] : bad[0];
+                    bad_s[i & 7][nth & 3][(warp - 2) * 2 + lane] = mine;
+                    if (mine) any_bad_s[i & 7] = 1;
+                }
                 ++nth;
                 proxy_fence();
                 __syncwarp();
@@ -401,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         }
     }
     } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     if (fine) {
         const int t = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -409,9 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         const float c = a.scale * 1.44269504088896341f;
         uint32_t s_uses = 0, o_uses = 0;
         for (int i = 0;; ++i) {
-            const int u = next_unit();
-            if (u < 0 || !ok) break;
-            const Unit x = unit_at<PAIR>(a, pre, u);
+            Unit x;
+            if (!next_unit(x)) break;
             const int nt = x.nt[t], limit = x.s.m - x.s.n + x.tok[t] + row;  // the last key this row sees
             float ref = kNegInf, sum = 0.f;  // weights are exp2((s - ref) c)
             for (int j = 0; j < nt; ++j) {
@@ -484,6 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                 tc_after();
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const bool any_bad = nt > 0 && *reinterpret_cast<volatile int*>(&any_bad_s[i & 7]) != 0;
             T* out = static_cast<T*>(a.out) + static_cast<long long>(x.s.q0 + x.tok[t] + row) * a.out_stride + x.head[t] * HD;
 #pragma unroll 1
             for (int b = 0; b < HD / 32; ++b) {
@@ -502,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                 if (row < x.rows[t]) {
                     // Values that the guard set aside, where this row sees them.
                     int nth = 0;
-                    for (int j = x.first_cut(); j < x.key_tiles; ++j) {
+                    for (int j = any_bad ? x.first_cut() : x.key_tiles; j < x.key_tiles; ++j) {
                         if (!x.cut(j)) continue;
                         for (int w = 0; w < 4; ++w) {
                             for (uint32_t bits = bad_s[i & 7][nth & 3][w]; bits; bits &= bits - 1) {

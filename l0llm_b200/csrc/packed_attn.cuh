@@ -69,11 +69,11 @@ __device__ __forceinline__ bool packed_scan(const PackedAttnParams& a, int* pre,
     return fine;
 }
 
-// Whether one of a pair of 16-bit values is an infinity or a NaN (every exponent bit set).
+// Whether one of eight 16-bit values is an infinity or a NaN: an exponent of ones carries into the bit above it.
 template <bool BF>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-    const uint32_t e = BF ? 0x7F80u : 0x7C00u;
-    return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ bool not_finite(const uint4& w) {
+    const uint32_t mask = BF ? 0x7F807F80u : 0x7C007C00u, one = BF ? 0x00800080u : 0x04000400u;
+    return ((((w.x & mask) + one) | ((w.y & mask) + one) | ((w.z & mask) + one) | ((w.w & mask) + one)) & 0x80008000u) != 0;
 }
 
 // o[0, 32) (f32 bits) += weight * value of one key, dims 32 b .. 32 b + 31, the weight worked out anew: for the few
