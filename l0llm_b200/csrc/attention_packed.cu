@@ -178,8 +178,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_s = smem;               // [2][TILE]
     uint8_t* kv_s = smem + 2 * TILE;   // [kRing][TILE]
-    int* pre = reinterpret_cast<int*>(kv_s + kRing * TILE);  // [count + 1] units before each sequence
-    __shared__ __align__(8) uint64_t bars[2 + 2 * kRing + 4 * 2 + kRing + 2 * kUnitSlots];
+    uint8_t* stage_s = kv_s + kRing * TILE;  // [8 softmax warps][32 rows of 64 bytes] of the epilogue
+    int* pre = reinterpret_cast<int*>(stage_s + 8 * 2048);  // [count + 1] units before each sequence
+    __shared__ __align__(8) uint64_t bars[2 + 2 * kRing + 5 * 2 + kRing + 2 * kUnitSlots];
     __shared__ Unit unit_s[kUnitSlots];
     __shared__ int scan_s[kThreads / 32];
     __shared__ unsigned long long rows_s;
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t bar0 = smem_addr(bars);
     const uint32_t q_full = bar0, q_empty = bar0 + 8, kv_full = bar0 + 16, kv_empty = kv_full + 8 * kRing;
-    const uint32_t s_full = kv_empty + 8 * kRing, p_ready = s_full + 16, o_full = p_ready + 16, o_empty = o_full + 16;
+    const uint32_t s_full = kv_empty + 8 * kRing, p_ready = s_full + 16, o_full = p_ready + 32, o_empty = o_full + 16;
     const uint32_t v_ok = o_empty + 16, drawn = v_ok + 8 * kRing, read = drawn + 8 * kUnitSlots;
 
     if (threadIdx.x == 0) {
@@ -204,7 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         }
         for (int t = 0; t < 2; ++t) {
             bar_init(s_full + 8 * t, 1);
-            bar_init(p_ready + 8 * t, kRows);
+            bar_init(p_ready + 16 * t, kRows);      // weights of keys 0-63 of a tile
+            bar_init(p_ready + 16 * t + 8, kRows);  // of keys 64-127
             bar_init(o_full + 8 * t, 1);
             bar_init(o_empty + 8 * t, kRows);
         }
@@ -344,13 +346,17 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                         have_v = true;
                     }
                     if (j == 0 && !wait_warp(o_empty + 8 * t, (o_uses[t]++ & 1) ^ 1)) break;
-                    if (!wait_warp(p_ready + 8 * t, p_uses[t]++ & 1)) break;
-                    tc_after();
                     const uint32_t v = smem_addr(kv_s) + st * TILE;
 #pragma unroll
-                    for (int i = 0; i < kRows / 16; ++i)
-                        mma_ts(tmem + 2 * kRows + t * HD, tmem + t * kRows + i * 8, n_major_desc(v + i * 2048), kIdescO,
-                               j > 0 || i > 0);
+                    for (int h = 0; h < 2; ++h) {
+                        if (!wait_warp(p_ready + 16 * t + 8 * h, p_uses[t] & 1)) break;
+                        tc_after();
+#pragma unroll
+                        for (int i = 4 * h; i < 4 * h + 4; ++i)
+                            mma_ts(tmem + 2 * kRows + t * HD, tmem + t * kRows + i * 8, n_major_desc(v + i * 2048), kIdescO,
+                                   j > 0 || i > 0);
+                    }
+                    ++p_uses[t];
                     if (t == (j < x.nt[1] ? 1 : 0)) tc_commit(kv_empty + 8 * st);
                     if (j + 1 < x.nt[t]) scores(t, j + 1);
                     else tc_commit(o_full + 8 * t);
@@ -425,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + t * kRows + lanes, o_at = tmem + 2 * kRows + t * HD + lanes;
         const float c = a.scale * 1.44269504088896341f;
+        uint8_t* stage = stage_s + (warp - 4) * 2048;
         uint32_t s_uses = 0, o_uses = 0;
         for (int i = 0;; ++i) {
             Unit x;
@@ -449,8 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
 #pragma unroll
-                    for (int b = 0; b < 4; ++b)
-                        top[b] = fmaxf(fmaxf(top[b], __uint_as_float(s[b][k])), __uint_as_float(s[b][k + 1]));
+                    for (int b = 0; b < 4; ++b) top[b] = fmaxf(fmaxf(top[b], __uint_as_float(s[b][k])), __uint_as_float(s[b][k + 1]));
                 }
                 const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 // The reference moves when it must: at the first keys seen, or when weights would pass 2^8.
@@ -489,11 +495,13 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                         w[k] = pack2<T>(y.x, y.y);
                     }
                     tmem_store16(s_at + 16 * b, w);
+                    if (b & 1) {
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        tc_before();
+                        bar_arrive(p_ready + 16 * t + 4 * (b - 1));
+                    }
                 }
                 sum += (add[0].x + add[0].y) + (add[1].x + add[1].y);
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                tc_before();
-                bar_arrive(p_ready + 8 * t);
             }
             if (x.rows[t] == 0 || !ok) continue;
             if (nt > 0) {
@@ -502,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const bool any_bad = nt > 0 && *reinterpret_cast<volatile int*>(&any_bad_s[i & 7]) != 0;
-            T* out = static_cast<T*>(a.out) + static_cast<long long>(x.s.q0 + x.tok[t] + row) * a.out_stride + x.head[t] * HD;
+            T* out = static_cast<T*>(a.out) + static_cast<long long>(x.s.q0 + x.tok[t] + (warp & 3) * 32) * a.out_stride + x.head[t] * HD;
 #pragma unroll 1
             for (int b = 0; b < HD / 32; ++b) {
                 uint32_t o[32];
@@ -526,20 +534,35 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                             for (uint32_t bits = bad_s[i & 7][nth & 3][w]; bits; bits &= bits - 1) {
                                 const int key = j * kRows + w * 32 + __ffs(bits) - 1;
                                 if (key > limit) break;
-                                add_value_share<T, HD>(a, x.s, x.head[t], x.tok[t] + row, key, c, ref == kNegInf ? 0.f : ref * c, b, o);
+                                const float f = weight_anew<T, HD>(a, x.s, x.head[t], x.tok[t] + row, key, c, ref == kNegInf ? 0.f : ref * c);
+                                const T* v = static_cast<const T*>(a.v) + static_cast<long long>(x.s.k0 + key) * a.v_stride +
+                                             x.head[t] / (a.nh / a.nkv) * HD + 32 * b;
+#pragma unroll
+                                for (int k = 0; k < 32; ++k)
+                                    o[k] = __float_as_uint(fmaf(f, load_as_float(v, DT<T>::id, k), __uint_as_float(o[k])));
                             }
                         }
                         ++nth;
                     }
+                }
+                // 32 rows of 64 bytes through shared memory, so that four lanes store one row's 64 bytes: a store of
+                // 16 bytes of 32 rows takes 32 turns of the memory pipe, one of 64 bytes of 8 rows takes 8.
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        uint4 w;
-                        w.x = pack2<T>(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
-                        w.y = pack2<T>(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
-                        w.z = pack2<T>(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
-                        w.w = pack2<T>(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
-                        *reinterpret_cast<uint4*>(out + 32 * b + k) = w;
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    uint4 w;
+                    w.x = pack2<T>(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
+                    w.y = pack2<T>(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
+                    w.z = pack2<T>(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
+                    w.w = pack2<T>(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = w;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = k * 8 + (lane >> 2), piece = lane & 3;
+                    const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
+                    if ((warp & 3) * 32 + r < x.rows[t])
+                        *reinterpret_cast<uint4*>(out + r * a.out_stride + 32 * b + piece * 8) = w;
                 }
                 __syncwarp();
             }
@@ -565,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
 template <bool BF, int HD, bool PAIR>
 l0b_status launch_tc(l0b_suite* s, l0b_device* d, const PackedAttnParams& a) {
     auto kernel = packed_tc_kernel<BF, HD, PAIR>;
-    constexpr size_t tiles = 1024 + static_cast<size_t>(2 + kRing) * (HD / 64) * kSub;
+    constexpr size_t tiles = 1024 + static_cast<size_t>(2 + kRing) * (HD / 64) * kSub + 8 * 2048;
     {
         static bool configured[64] = {};
         static std::mutex mu;

@@ -76,19 +76,16 @@ __device__ __forceinline__ bool not_finite(const uint4& w) {
     return ((((w.x & mask) + one) | ((w.y & mask) + one) | ((w.z & mask) + one) | ((w.w & mask) + one)) & 0x80008000u) != 0;
 }
 
-// o[0, 32) (f32 bits) += weight * value of one key, dims 32 b .. 32 b + 31, the weight worked out anew: for the few
-// values that are not finite in tiles that the mask cuts.
+// The weight exp2((q . k) c - shift) of one key for one query row, worked out anew: for the few values that are not
+// finite in tiles that the mask cuts.
 template <typename T, int HD>
-__device__ __noinline__ void add_value_share(const PackedAttnParams& a, const PackedSeq& s, int head, int row, int key, float c,
-                                             float shift, int b, uint32_t (&o)[32]) {
-    const int kvh = head / (a.nh / a.nkv);
-    const T* k = static_cast<const T*>(a.k) + static_cast<long long>(s.k0 + key) * a.k_stride + kvh * HD;
-    const T* v = static_cast<const T*>(a.v) + static_cast<long long>(s.k0 + key) * a.v_stride + kvh * HD + 32 * b;
+__device__ __noinline__ float weight_anew(const PackedAttnParams& a, const PackedSeq& s, int head, int row, int key, float c,
+                                          float shift) {
+    const T* k = static_cast<const T*>(a.k) + static_cast<long long>(s.k0 + key) * a.k_stride + head / (a.nh / a.nkv) * HD;
     const long long q = static_cast<long long>(s.q0 + row) * a.q_stride + static_cast<long long>(head) * HD;
     float dot = 0.f;
     for (int d = 0; d < HD; ++d) dot = fmaf(load_as_float(a.q, a.q_dtype, q + d), load_as_float(k, DT<T>::id, d), dot);
-    const float w = exp2f(dot * c - shift);
-    for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(fmaf(w, load_as_float(v, DT<T>::id, d), __uint_as_float(o[d])));
+    return exp2f(dot * c - shift);
 }
 
 }  // namespace l0b
