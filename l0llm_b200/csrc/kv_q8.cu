@@ -7,10 +7,10 @@
 // the rows are read once and the codes written once; both are bound by HBM.
 //
 // scale = f32(max / 127), never below the old one where slots of the block below the piece are kept.
-// code = rint(x / scale) of the exact quotient: q = rint(x * (1 / scale)) may be one off next to a half, and
-// the residual x - q * scale decides. In f32 fma that residual is exact wherever it is near scale / 2 (x and
-// q * scale are multiples of ulp(scale) there, or x is below scale and within a factor of two of it), so
-// 2 |r| compares with scale as the real numbers do; a tie goes to the even code.
+// code = rint(x / scale) of the exact quotient: the nearest integer q to x * (1 / scale) may be one off next to a half,
+// and the residual x - q * scale decides. In f32 fma that residual is exact wherever it is near scale / 2 (x and
+// q * scale are multiples of ulp(scale) there, or x is below scale and within a factor of two of it), so |r| compares
+// with scale / 2 as the real numbers do; a tie goes to the even code.
 #include "ops.cuh"
 #include "packed.cuh"
 
@@ -20,34 +20,64 @@ namespace {
 
 constexpr int kPer = 32;  // values of a piece per thread: threads = block * hd / 32
 
-__device__ __forceinline__ int code_of(float x, float scale, float inv) {
-    float q = rintf(x * inv);
-    const float r = fmaf(-q, scale, x), twice = 2.f * fabsf(r);
-    const float toward = r < 0.f ? -1.f : 1.f;
-    if (twice > scale || (twice == scale && (static_cast<int>(q) & 1))) q += toward;
-    return static_cast<int>(fminf(127.f, fmaxf(-127.f, q)));
-}
-
-// The same by f64, where 1 / scale has no f32 or x is an old code times its old scale: a quotient of at most
-// 2^31 / 2^24 that is not a half is further from it than f64's rounding.
+// rint(x / scale) of the exact quotient by f64, for scales whose reciprocal is no normal f32 and for x an old code
+// times its old scale: a quotient of numbers of 31 and 24 bits that is not a half is further from one than f64 rounds.
 __device__ __forceinline__ int code_of_f64(double x, float scale) {
     return static_cast<int>(fmin(127.0, fmax(-127.0, rint(x / static_cast<double>(scale)))));
 }
 
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const uint32_t* w, int i) {  // values 2 i, 2 i + 1
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else return DT<T>::id == L0B_F16 ? half2_bits_to_float2(w[i]) : bf162_bits_to_float2(w[i]);
+}
+
+// Codes of the slots [0, kept) of a block from one scale to another.
+__device__ __noinline__ void rescale_kept(int8_t* block, int kvd, int hd_log, int kept, float old, float scale, bool fine) {
+    for (int e = threadIdx.x * 8; e < kept << hd_log; e += blockDim.x * 8) {
+        uint2* at = reinterpret_cast<uint2*>(block + static_cast<long long>(e >> hd_log) * kvd + (e & ((1 << hd_log) - 1)));
+        const uint2 was = *at;
+        uint32_t w[2] = {was.x, was.y};
+        for (int k = 0; k < 2; ++k) {
+            uint32_t u = 0;
+            for (int i = 0; i < 32; i += 8) {
+                const int c = static_cast<int8_t>(w[k] >> i);
+                u |= (static_cast<uint32_t>(fine ? code_of_f64(c * static_cast<double>(old), scale) : 0) & 0xFFu) << i;
+            }
+            w[k] = u;
+        }
+        *at = make_uint2(w[0], w[1]);
+    }
+}
+
+// Codes of a piece of n rows by f64, or 0 where the scale is 0 or not finite; the rows are read again.
 template <typename T, int HD>
-__global__ void __launch_bounds__(512) kv_q8_store_kernel(const KvQ8Params p, int rows_per_cta) {
+__device__ __noinline__ void store_slowly(const T* src, long long stride, int8_t* dst, int kvd, int n, float scale, bool fine) {
+    for (int e = threadIdx.x; e < n * HD; e += blockDim.x) {
+        const int r = e / HD, c = e % HD;
+        dst[static_cast<long long>(r) * kvd + c] =
+            static_cast<int8_t>(fine ? code_of_f64(load_as_float(src, DT<T>::id, r * stride + c), scale) : 0);
+    }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p, int rows_per_cta) {
+    constexpr int WORDS = 8 * sizeof(T) / 4;  // of eight values
     __shared__ unsigned red[32];
-    const int head = blockIdx.y >> 1, which = blockIdx.y & 1;
+    // The heads of the same rows side by side: together they read and write whole rows while their DRAM pages are open.
+    const int range = blockIdx.x / (2 * p.nkv), hw = blockIdx.x - range * 2 * p.nkv, head = hw >> 1, which = hw & 1;
     const int kvd = p.nkv * HD;
     const T* src = static_cast<const T*>(which ? p.v : p.k) + head * HD;
     const long long stride = which ? p.v_stride : p.k_stride;
     int8_t* cache = (which ? p.vc : p.kc) + head * HD;
     float* scales = (which ? p.vs : p.ks) + head;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+    const int block_log = 31 - __clz(p.block);
+    const int row0 = tid / (HD / 8), col = tid % (HD / 8) * 8, step = blockDim.x / (HD / 8);
     pdl_wait();
     pdl_launch_dependents();
 
-    const int t0 = blockIdx.x * rows_per_cta, t1 = min(p.tokens, t0 + rows_per_cta);
+    const int t0 = range * rows_per_cta, t1 = min(p.tokens, t0 + rows_per_cta);
     int seq = p.starts ? block_find_sequence(p.starts, p.count, t0) : t0;
     if (seq < 0) seq = 0;  // rows before the first sequence; a sequence may still start inside the range
     for (; seq < p.count; ++seq) {
@@ -62,133 +92,161 @@ __global__ void __launch_bounds__(512) kv_q8_store_kernel(const KvQ8Params p, in
         const int stop = min(end - first, p.max_seq - pos) + pos;  // past the sequence's last new slot
         // Leaders of this sequence in [t0, t1): its first row, then every row that opens a block.
         long long t = first;
-        if (t < t0) t = t0 + (p.block - (pos + static_cast<long long>(t0 - first)) % p.block) % p.block;
+        if (t < t0) t = t0 + (-(pos + (t0 - first)) & (p.block - 1));
         while (t < min(end, t1) && pos + (t - first) < stop) {
             const int slot = static_cast<int>(pos + (t - first));
-            const int blk = slot / p.block, base = blk * p.block;
-            const int last = min(base + p.block, stop);  // past the piece's last new slot
-            const int n = last - slot;
-            // Values of the piece: thread holds four groups of eight, group g at element (g * threads + tid) * 8.
-            float x[4][8];
-            unsigned top = 0;
+            const int blk = slot >> block_log, base = blk << block_log;
+            const int n = min(base + p.block, stop) - slot, kept = slot - base;
+            // Values of the piece: a thread holds eight columns from `col` on of four rows, `step` apart.
+            const T* from = src + (t + row0) * stride + col;
+            uint32_t w[4][WORDS];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int e = (g * blockDim.x + tid) * 8, r = e / HD, c = e % HD;
-                if (r < n) {
-                    load8_f32(src + (t + r) * stride + c, x[g]);
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[g][i] = 0.f;
+                for (int i = 0; i < WORDS; i += 4) {
+                    uint4 u = make_uint4(0, 0, 0, 0);
+                    if (row0 + g * step < n) u = ld_stream_v4(from + i * 4 / static_cast<int>(sizeof(T)));
+                    w[g][i] = u.x;
+                    w[g][i + 1] = u.y;
+                    w[g][i + 2] = u.z;
+                    w[g][i + 3] = u.w;
                 }
+                from += step * stride;
+            }
+            float* sp = scales + (static_cast<long long>(seq) * p.blocks + blk) * p.nkv;
+            const float old = kept > 0 ? *sp : 0.f;
+            unsigned top = 0;  // the largest magnitude's bits: an infinity is above every number, a NaN above that
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[g][i]) & 0x7FFFFFFFu);
+            for (int g = 0; g < 4; ++g) {
+#pragma unroll
+                for (int i = 0; i < WORDS; i += 2) {
+                    if constexpr (sizeof(T) == 4) top = __vimax3_u32(top, w[g][i] & 0x7FFFFFFFu, w[g][i + 1] & 0x7FFFFFFFu);
+                    else top = __vimax3_u16x2(top, w[g][i] & 0x7FFF7FFFu, w[g][i + 1] & 0x7FFF7FFFu);
+                }
+            }
+            if constexpr (sizeof(T) == 2) {  // the larger half, as f32 bits
+                const float2 both = pair_of<T>(&top, 0);
+                top = max(__float_as_uint(both.x), __float_as_uint(both.y));
             }
             top = __reduce_max_sync(0xffffffffu, top);
             __syncthreads();
             if (lane == 0) red[warp] = top;
-            __syncthreads();
+            __syncthreads();  // and every thread has read the old scale
             top = __reduce_max_sync(0xffffffffu, lane < warps ? red[lane] : 0u);
-            float* sp = scales + (static_cast<long long>(seq) * p.blocks + blk) * p.nkv;
-            float scale = __fdiv_rn(__uint_as_float(top), 127.f), old = 0.f;
-            const int kept = slot - base;
-            if (kept > 0) {
-                old = *sp;
-                const unsigned ob = __float_as_uint(old) & 0x7FFFFFFFu, nb = __float_as_uint(scale);
-                scale = __uint_as_float(max(ob, nb));
-            }
+            float scale = __fdiv_rn(__uint_as_float(top), 127.f);
+            if (kept > 0) scale = __uint_as_float(max(__float_as_uint(old) & 0x7FFFFFFFu, __float_as_uint(scale)));
             const bool fine = scale > 0.f && scale < __int_as_float(0x7F800000);
             int8_t* dst = cache + (static_cast<long long>(seq) * p.max_seq + base) * kvd;
-            if (kept > 0 && __float_as_uint(scale) != __float_as_uint(old)) {
-                for (int e = tid * 8; e < kept * HD; e += blockDim.x * 8) {
-                    const int r = e / HD, c = e % HD;
-                    uint2* at = reinterpret_cast<uint2*>(dst + static_cast<long long>(r) * kvd + c);
-                    const uint2 was = *at;
-                    uint32_t w[2] = {was.x, was.y};
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        uint32_t u = 0;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int c8 = static_cast<int8_t>(w[k] >> (8 * i));
-                            const int q = fine ? code_of_f64(c8 * static_cast<double>(old), scale) : 0;
-                            u |= (static_cast<uint32_t>(q) & 0xFFu) << (8 * i);
-                        }
-                        w[k] = u;
-                    }
-                    *at = make_uint2(w[0], w[1]);
-                }
-            }
-            const float inv = 1.f / scale;
-            const bool quick = fine && scale > 1e-36f;  // 1 / scale and twice the residual are normal numbers
+            if (kept > 0 && __float_as_uint(scale) != __float_as_uint(old))
+                rescale_kept(dst, kvd, HD == 128 ? 7 : 6, kept, old, scale, fine);
             dst += static_cast<long long>(kept) * kvd;
+            if (fine && scale > 1e-36f) {  // the reciprocal and every residual next to a half are normal numbers
+                const float inv = 1.f / scale, half = 0.5f * scale;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int e = (g * blockDim.x + tid) * 8, r = e / HD, c = e % HD;
-                if (r >= n) continue;
-                uint32_t w[2] = {0, 0};
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t q[8];
+                    float worst = 0.f, res[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int q = quick ? code_of(x[g][i], scale, inv) : fine ? code_of_f64(x[g][i], scale) : 0;
-                    w[i >> 2] |= (static_cast<uint32_t>(q) & 0xFFu) << (8 * (i & 3));
+                    for (int i = 0; i < 4; ++i) {
+                        // 1.5 2^23 + the nearest integer: its low byte is the code
+                        const float2 x = pair_of<T>(w[g], i);
+                        const float n0 = fmaf(x.x, inv, 12582912.f), n1 = fmaf(x.y, inv, 12582912.f);
+                        res[2 * i] = fmaf(12582912.f - n0, scale, x.x);
+                        res[2 * i + 1] = fmaf(12582912.f - n1, scale, x.y);
+                        q[2 * i] = __float_as_uint(n0);
+                        q[2 * i + 1] = __float_as_uint(n1);
+                        worst = fmaxf(fmaxf(worst, fabsf(res[2 * i])), fabsf(res[2 * i + 1]));
+                    }
+                    // a branch of the warp: as predicated code this was a third of the kernel's instructions
+                    if (__any_sync(0xffffffffu, worst >= half)) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float d = fabsf(res[i]);
+                            if (d > half || (d == half && (q[i] & 1))) q[i] += res[i] < 0.f ? -1 : 1;
+                        }
+                    }
+                    uint2 out;
+                    out.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+                    out.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+                    if (row0 + g * step < n)
+                        *reinterpret_cast<uint2*>(dst + static_cast<long long>(row0 + g * step) * kvd + col) = out;
                 }
-                *reinterpret_cast<uint2*>(dst + static_cast<long long>(r) * kvd + c) = make_uint2(w[0], w[1]);
+            } else {
+                store_slowly<T, HD>(src + t * stride, stride, dst, kvd, n, scale, fine);
             }
-            __syncthreads();  // every thread has read the old scale
             if (tid == 0) *sp = scale;
             t += n;
         }
     }
 }
 
-// Load. A CTA takes `rows` packed rows; each thread turns sixteen codes at a time into values. Bound by HBM.
+// Load. A warp takes a run of packed rows, K and V of each: 128 or 256 codes a step into 512 contiguous bytes. Bound
+// by HBM.
 template <typename T>
 __global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p, int rows) {
-    __shared__ int slot_of[32], seq_of[32];
+    constexpr int VEC = 16 / sizeof(T);  // codes of a thread's step: 16 bytes out
     pdl_wait();
     pdl_launch_dependents();
-    const int t0 = blockIdx.x * rows, n = min(rows, p.tokens - t0);
-    const int s0 = p.starts ? block_find_sequence(p.starts, p.count, t0) : t0;
-    if (threadIdx.x < n) {
-        const int t = t0 + threadIdx.x;
-        int seq = p.starts ? max(s0, 0) : t, slot = -1;
-        if (p.starts) {
-            while (seq + 1 < p.count && p.starts[seq + 1] <= t) ++seq;
-        }
-        const int first = p.starts ? p.starts[seq] : seq, end = p.starts ? p.starts[seq + 1] : seq + 1;
-        if (t >= first && t < end) {
-            const int pos = p.positions[seq];
-            if (pos < 0 || first < 0 || end > p.tokens || pos >= p.max_seq - (t - first)) flag_bad_index(p.error);
-            if (pos >= 0 && pos < p.max_seq - (t - first)) slot = pos + (t - first);
-        }
-        slot_of[threadIdx.x] = slot;
-        seq_of[threadIdx.x] = seq;
+    const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int kvd = p.nkv * p.hd, hd_log = p.hd == 128 ? 7 : 6, block_log = 31 - __clz(p.block);
+    int t = warp * rows;
+    const int t1 = min(p.tokens, t + rows);
+    if (t >= t1) return;
+    int seq = t, first = t, end = t, pos = 0;
+    if (p.starts) {  // the last sequence that starts at or before the run
+        seq = -1;
+        for (int i = lane; __any_sync(0xffffffffu, i < p.count); i += 32)
+            seq += __popc(__ballot_sync(0xffffffffu, i < p.count && __ldg(p.starts + i) <= t));
+        first = end = INT32_MIN;
+        --seq;
     }
-    __syncthreads();
-    const int kvd = p.nkv * p.hd, per_row = kvd / 16;
-    for (int e = threadIdx.x; e < n * per_row * 2; e += 256) {
-        const int which = e >= n * per_row;
-        const int i = which ? e - n * per_row : e;
-        const int r = i / per_row, c = (i - r * per_row) * 16;
-        const int slot = slot_of[r], seq = seq_of[r];
-        if (slot < 0) continue;
-        const int8_t* src = (which ? p.vc : p.kc) + (static_cast<long long>(seq) * p.max_seq + slot) * kvd + c;
-        const float scale = (which ? p.vs : p.ks)[(static_cast<long long>(seq) * p.blocks + slot / p.block) * p.nkv + c / p.hd];
-        const uint4 w4 = ld_stream_v4(src);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-        T* dst = static_cast<T*>(const_cast<void*>(which ? p.v : p.k)) + (t0 + r) * (which ? p.v_stride : p.k_stride) + c;
+    for (; t < t1; ++t) {
+        if (!p.starts) {
+            seq = first = t;
+            end = t + 1;
+            pos = __ldg(p.positions + t);
+        } else if (t >= end) {  // on to the sequence of this row
+            do ++seq;
+            while (seq < p.count && (seq < 0 || __ldg(p.starts + seq + 1) <= t));
+            if (seq >= p.count) return;
+            first = __ldg(p.starts + seq);
+            end = __ldg(p.starts + seq + 1);
+            pos = __ldg(p.positions + seq);
+        }
+        if (t < first) continue;
+        const bool fits = pos >= 0 && pos < p.max_seq - (t - first);
+        if (lane == 0 && (!fits || first < 0 || end > p.tokens)) flag_bad_index(p.error);
+        if (!fits) continue;
+        const int slot = pos + (t - first);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float v[8];
+        for (int which = 0; which < 2; ++which) {
+            const int8_t* src = (which ? p.vc : p.kc) + (static_cast<long long>(seq) * p.max_seq + slot) * kvd;
+            const float* scales = (which ? p.vs : p.ks) + (static_cast<long long>(seq) * p.blocks + (slot >> block_log)) * p.nkv;
+            T* dst = static_cast<T*>(const_cast<void*>(which ? p.v : p.k)) + t * (which ? p.v_stride : p.k_stride);
+#pragma unroll 4
+            for (int c = lane * VEC; c < kvd; c += 32 * VEC) {
+                const float scale = __ldg(scales + (c >> hd_log));
+                float v[8];
+                uint32_t w[2];
+                if constexpr (VEC == 4) {
+                    w[0] = __ldg(reinterpret_cast<const unsigned*>(src + c));
+                } else {
+                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(src + c));
+                    w[0] = u.x;
+                    w[1] = u.y;
+                }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float2 a, b;
-                dequant_i8x4(w[2 * h + j], a, b);
-                v[4 * j] = a.x * scale;
-                v[4 * j + 1] = a.y * scale;
-                v[4 * j + 2] = b.x * scale;
-                v[4 * j + 3] = b.y * scale;
+                for (int j = 0; j < VEC / 4; ++j) {
+                    float2 a, b;
+                    dequant_i8x4(w[j], a, b);
+                    v[4 * j] = a.x * scale;
+                    v[4 * j + 1] = a.y * scale;
+                    v[4 * j + 2] = b.x * scale;
+                    v[4 * j + 3] = b.y * scale;
+                }
+                if constexpr (VEC == 4) *reinterpret_cast<float4*>(dst + c) = make_float4(v[0], v[1], v[2], v[3]);
+                else store8(dst + c, v);
             }
-            store8(dst + 8 * h, v);
         }
     }
 }
@@ -201,17 +259,18 @@ l0b_status store_as(l0b_device* d, const KvQ8Params& p) {
     const long long pieces = static_cast<long long>(p.tokens) * p.nkv * 2;
     int rows = p.starts ? p.block : 1;
     while (rows > 1 && pieces / rows < 8LL * d->sm_count) rows >>= 1;
-    const dim3 grid((p.tokens + rows - 1) / rows, p.nkv * 2);
-    L0B_REQUIRE(p.nkv <= 32767, L0B_ERR_OUT_OF_RANGE, "KV heads %d exceed 32767", p.nkv);
+    const long long ctas = (static_cast<long long>(p.tokens) + rows - 1) / rows * p.nkv * 2;
+    L0B_REQUIRE(ctas <= INT32_MAX, L0B_ERR_OUT_OF_RANGE, "%d rows of %d KV heads are too many for one call", p.tokens, p.nkv);
+    const dim3 grid(static_cast<unsigned>(ctas));
     if (p.hd == 64) return d->launch(kv_q8_store_kernel<T, 64>, grid, dim3(threads), 0, p, rows);
     return d->launch(kv_q8_store_kernel<T, 128>, grid, dim3(threads), 0, p, rows);
 }
 
 template <typename T>
 l0b_status load_as(l0b_device* d, const KvQ8Params& p) {
-    int rows = 32;
-    while (rows > 1 && p.tokens / rows < 4 * d->sm_count) rows >>= 1;
-    return d->launch(kv_q8_load_kernel<T>, dim3((p.tokens + rows - 1) / rows), dim3(256), 0, p, rows);
+    // Rows a warp: one, until 64 warps an SM have more than that.
+    const int rows = (p.tokens + 64 * d->sm_count - 1) / (64 * d->sm_count);
+    return d->launch(kv_q8_load_kernel<T>, dim3((p.tokens + 8 * rows - 1) / (8 * rows)), dim3(256), 0, p, rows);
 }
 
 }  // namespace
