@@ -123,30 +123,42 @@ __global__ void __launch_bounds__(128, 2) packed_f32_kernel(const PackedAttnPara
     };
     if (tiles > 0) load(0, 0);
 
-    // Query terms: a warp's own 16 rows, a row at a time, four lanes' worth of dims each.
+    // Query terms: a warp's own 16 rows, eight rows' loads in flight, a row spread over the lanes.
     if (tid < 4) bad_s[tid >> 1][tid & 1] = 0;
-    for (int r = 0; r < 16; ++r) {
-        const int row = warp * 16 + r;
-        float x[HD / 32];
-        const float* q = static_cast<const float*>(p.q) + static_cast<long long>(s.q0 + tok + min(row, rows - 1)) * p.q_stride +
-                         static_cast<long long>(head) * HD + lane * (HD / 32);
+    for (int r0 = 0; r0 < 16; r0 += 8) {
+        float x[8][HD / 32];
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) x[i] = q[i];
-        float top = 0.f;
+        for (int r = 0; r < 8; ++r) {
+            const float* q = static_cast<const float*>(p.q) +
+                             static_cast<long long>(s.q0 + tok + min(warp * 16 + r0 + r, rows - 1)) * p.q_stride +
+                             static_cast<long long>(head) * HD + lane * (HD / 32);
+            if constexpr (HD == 128) {
+                const float4 y = __ldg(reinterpret_cast<const float4*>(q));
+                x[r][0] = y.x; x[r][1] = y.y; x[r][2] = y.z; x[r][3] = y.w;
+            } else {
+                const float2 y = __ldg(reinterpret_cast<const float2*>(q));
+                x[r][0] = y.x; x[r][1] = y.y;
+            }
+        }
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) top = fmaxf(top, fabsf(x[i]));
-        top = warp_max(top);
-        const int bits = top > 0.f && top < __int_as_float(0x7F800000) ? min(13 - ilogbf(top), 126) : 0;  // to [2^13, 2^14)
-        const float up = ldexpf(1.f, bits);
-        if (lane == 0) factor_s[row] = ldexpf(p.scale * 1.44269504088896341f, -bits);
+        for (int r = 0; r < 8; ++r) {
+            const int row = warp * 16 + r0 + r;
+            float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < HD / 32; i += 2) {
-            uint32_t term[NT];
-            split<T>(x[i] * up, x[i + 1] * up, term);
-            const int d = lane * (HD / 32) + i;  // dim
+            for (int i = 0; i < HD / 32; ++i) top = fmaxf(top, fabsf(x[r][i]));
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+            const int bits = top > 0.f && top < __int_as_float(0x7F800000) ? min(13 - ilogbf(top), 126) : 0;  // to [2^13, 2^14)
+            const float up = ldexpf(1.f, bits);
+            if (lane == 0) factor_s[row] = ldexpf(p.scale * 1.44269504088896341f, -bits);
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                *reinterpret_cast<uint32_t*>(q_s + n * TILE + row * RB + (((d >> 3) ^ (row & 7)) << 4) + (d & 7) * 2) = term[n];
+            for (int i = 0; i < HD / 32; i += 2) {
+                uint32_t term[NT];
+                split<T>(x[r][i] * up, x[r][i + 1] * up, term);
+                const int d = lane * (HD / 32) + i;  // dim
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    *reinterpret_cast<uint32_t*>(q_s + n * TILE + row * RB + (((d >> 3) ^ (row & 7)) << 4) + (d & 7) * 2) = term[n];
+            }
         }
     }
     __syncwarp();
@@ -199,15 +211,19 @@ __global__ void __launch_bounds__(128, 2) packed_f32_kernel(const PackedAttnPara
                 const int r = warp * 16 + (lane & 15), c = 2 * kk + (lane >> 4);
                 load_4x8x8<false>(a[i], smem_addr(q_s) + i * TILE + r * RB + ((c ^ (r & 7)) << 4));
             }
+            uint32_t b[4][4];
 #pragma unroll
-            for (int n = 0; n < 8; n += 2) {
-                const int r = n * 8 + (lane & 7) + ((lane >> 4) << 3), c = 2 * kk + ((lane >> 3) & 1);
-                uint32_t b[4];
-                load_4x8x8<false>(b, smem_addr(kt) + r * RB + ((c ^ (r & 7)) << 4));
+            for (int n = 0; n < 4; ++n) {
+                const int r = n * 16 + (lane & 7) + ((lane >> 4) << 3), c = 2 * kk + ((lane >> 3) & 1);
+                load_4x8x8<false>(b[n], smem_addr(kt) + r * RB + ((c ^ (r & 7)) << 4));
+            }
+            // small terms first; eight sums in turn, so that no MMA waits for the one before it
 #pragma unroll
-                for (int i = NT - 1; i >= 0; --i) {  // small terms first
-                    mma<T>(sc[n], a[i], b[0], b[1]);
-                    mma<T>(sc[n + 1], a[i], b[2], b[3]);
+            for (int i = NT - 1; i >= 0; --i) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    mma<T>(sc[2 * n], a[i], b[n][0], b[n][1]);
+                    mma<T>(sc[2 * n + 1], a[i], b[n][2], b[n][3]);
                 }
             }
         }
@@ -252,23 +268,29 @@ __global__ void __launch_bounds__(128, 2) packed_f32_kernel(const PackedAttnPara
             }
         }
 #pragma unroll
-        for (int n = 0; n < HD / 8; n += 2) {
-            float acc[2][4];
+        for (int n = 0; n < HD / 8; n += 8) {
+            float acc[8][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+            for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
-                const int r = 16 * kk + (lane & 15), c = n + (lane >> 4);
-                uint32_t b[4];
-                load_4x8x8<true>(b, smem_addr(vt) + r * RB + ((c ^ (r & 7)) << 4));
+                uint32_t b[4][4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int r = 16 * kk + (lane & 15), c = n + 2 * q + (lane >> 4);
+                    load_4x8x8<true>(b[q], smem_addr(vt) + r * RB + ((c ^ (r & 7)) << 4));
+                }
 #pragma unroll
                 for (int i = NT - 1; i >= 0; --i) {
-                    mma<T>(acc[0], w[kk][i], b[0], b[1]);
-                    mma<T>(acc[1], w[kk][i], b[2], b[3]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        mma<T>(acc[2 * q], w[kk][i], b[q][0], b[q][1]);
+                        mma<T>(acc[2 * q + 1], w[kk][i], b[q][2], b[q][3]);
+                    }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < 8; ++i) {
                 o[n + i][0] = fmaf(o[n + i][0], keep[0], acc[i][0]);
                 o[n + i][1] = fmaf(o[n + i][1], keep[0], acc[i][1]);
                 o[n + i][2] = fmaf(o[n + i][2], keep[1], acc[i][2]);
