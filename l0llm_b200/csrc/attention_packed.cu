@@ -29,92 +29,22 @@
 #include "packed.cuh"
 #include "packed_attn.cuh"
 #include "suite.h"
+#include "tcgen05.cuh"
 #include "tma.cuh"
 
 namespace l0b {
 
 namespace {
 
-constexpr int kRows = 128;     // query rows and keys of a tile
 constexpr int kRing = 4;       // K and V tiles in shared memory
 constexpr int kUnitSlots = 4;  // drawn units in flight
 constexpr int kThreads = 384;
-constexpr int kSub = kRows * 128;  // bytes of 128 rows of 64 16-bit columns, one 128-byte-swizzled block
 
 struct PackedLaunch {
     CUtensorMap qmap, kmap, vmap;  // [rows, heads * hd], box {64, 128}
     PackedAttnParams a;
     unsigned* counters;  // [0] units drawn beyond each CTA's first, [1] CTAs done; zero at rest
 };
-
-__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-// The MMA warp runs its loop whole and elects the issuing thread in each of these: in a branch of one thread the
-// compiler moved every operand to a uniform register per MMA, and eight MMAs took 820 cycles to issue, not 512.
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
-        : "memory");
-}
-// D (+)= A B^T, A and B in shared memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
-        : "memory");
-}
-// D (+)= A B, A in tensor memory.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
-        : "memory");
-}
-// Operand blocks of 128-byte swizzled rows. K-major (Q, K): eight-row groups 1024 bytes apart. N-major (V): the same
-// groups along the keys, blocks of 64 columns kSub apart.
-__device__ __forceinline__ uint64_t k_major_desc(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ uint64_t n_major_desc(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(kSub >> 4) << 16) | (64ull << 32) |
-           (1ull << 46) | (2ull << 61);
-}
-
-__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(addr));
-}
-// Waits for this thread's tensor-memory loads; the registers pass through, so no use of them moves above it.
-__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-          "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-          "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-          "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
-}
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-
 
 // One unit, worked out by the drawing thread and handed on in shared memory.
 struct Unit {
@@ -170,10 +100,7 @@ template <bool BF, int HD, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_constant__ PackedLaunch L) {
     using T = typename std::conditional<BF, __nv_bfloat16, __half>::type;
     constexpr int BLOCKS = HD / 64, TILE = BLOCKS * kSub;
-    constexpr uint32_t kIdescS = (1u << 4) | (static_cast<uint32_t>(BF) << 7) | (static_cast<uint32_t>(BF) << 10) |
-                                 (static_cast<uint32_t>(kRows >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
-    constexpr uint32_t kIdescO = (1u << 4) | (static_cast<uint32_t>(BF) << 7) | (static_cast<uint32_t>(BF) << 10) | (1u << 16) |
-                                 (static_cast<uint32_t>(HD >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+    constexpr uint32_t kIdescS = mma_idesc(BF, kRows, false), kIdescO = mma_idesc(BF, HD, true);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_s = smem;               // [2][TILE]
@@ -383,31 +310,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                     continue;
                 }
                 uint8_t* v = kv_s + st * TILE;
-                // A row takes LANES lanes of 16 bytes; a warp looks at AT_ONCE rows a step, eight steps in flight.
-                constexpr int LANES = BLOCKS * 8, AT_ONCE = 32 / LANES;
-                const int live = x.s.m - j * kRows, sub = lane / LANES, c = lane % LANES, base = (warp - 2) * 64;
-                uint32_t bad[2] = {0, 0};
-#pragma unroll 1
-                for (int r0 = 0; r0 < 64; r0 += 8 * AT_ONCE) {
-                    uint8_t* at = v + (c >> 3) * kSub + (base + r0 + sub) * 128 + (c & 7) * 16;
-                    uint32_t odd = 0;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(at + k * AT_ONCE * 128);
-                        odd |= static_cast<uint32_t>(not_finite<BF>(w) && base + r0 + k * AT_ONCE + sub < live) << k;
-                    }
-                    if (!__any_sync(0xffffffffu, odd != 0) && base + r0 + 8 * AT_ONCE <= live) continue;
-                    for (int k = 0; k < 8; ++k) {
-                        const uint32_t hit = __ballot_sync(0xffffffffu, (odd >> k) & 1);
-                        const uint32_t row_mask = (1u << LANES) - 1u;
-                        if (((hit >> (sub * LANES)) & row_mask) || base + r0 + k * AT_ONCE + sub >= live)
-                            *reinterpret_cast<uint4*>(at + k * AT_ONCE * 128) = make_uint4(0, 0, 0, 0);
-                        for (int q = 0; q < AT_ONCE; ++q) {
-                            const int r = r0 + k * AT_ONCE + q;
-                            if ((hit >> (q * LANES)) & row_mask) bad[r >> 5] |= 1u << (r & 31);
-                        }
-                    }
-                }
+                uint32_t bad[2];
+                guard_rows<BF, BLOCKS>(v, (warp - 2) * 64, x.s.m - j * kRows, lane, bad);
                 if (lane < 2) {
                     const uint32_t mine = lane ? bad[1] : bad[0];
                     bad_s[i & 7][nth & 3][(warp - 2) * 2 + lane] = mine;
@@ -622,10 +526,10 @@ l0b_status launch_as(l0b_suite* s, l0b_device* d, const PackedAttnParams& a) {
 }  // namespace
 
 l0b_status k_attention_packed(l0b_suite* s, l0b_device* d, const PackedAttnParams& p) {
-    if (p.q_dtype == L0B_F32) return k_attention_packed_f32(s, d, p);
     // Units are counted in 32 bits: blocks of rows times heads.
     L0B_REQUIRE((static_cast<long long>(p.tokens) / kRows + p.count) * p.nh <= INT32_MAX, L0B_ERR_OUT_OF_RANGE,
                 "%d rows of %d heads are too many for one call", p.tokens, p.nh);
+    if (p.q_dtype == L0B_F32) return k_attention_packed_f32(s, d, p);
     return p.kv_dtype == L0B_BF16 ? launch_as<true>(s, d, p) : launch_as<false>(s, d, p);
 }
 

@@ -4,6 +4,7 @@
 
 #include "ops.cuh"
 #include "packed.cuh"
+#include "tcgen05.cuh"
 
 namespace l0b {
 
@@ -74,6 +75,37 @@ template <bool BF>
 __device__ __forceinline__ bool not_finite(const uint4& w) {
     const uint32_t mask = BF ? 0x7F807F80u : 0x7C007C00u, one = BF ? 0x00800080u : 0x04000400u;
     return ((((w.x & mask) + one) | ((w.y & mask) + one) | ((w.z & mask) + one) | ((w.w & mask) + one)) & 0x80008000u) != 0;
+}
+
+// Makes 64 value rows of a cut tile, base on, safe for weights of 0, by one warp: rows from `live` on (another sequence's)
+// and rows with an infinity or a NaN become zeros; the latter are noted in bad. v: BLOCKS swizzled blocks of 64 columns.
+template <bool BF, int BLOCKS>
+__device__ __forceinline__ void guard_rows(uint8_t* v, int base, int live, int lane, uint32_t (&bad)[2]) {
+    // A row takes LANES lanes of 16 bytes; the warp looks at AT_ONCE rows a step, eight steps in flight.
+    constexpr int LANES = BLOCKS * 8, AT_ONCE = 32 / LANES;
+    const int sub = lane / LANES, c = lane % LANES;
+    bad[0] = bad[1] = 0;
+#pragma unroll 1
+    for (int r0 = 0; r0 < 64; r0 += 8 * AT_ONCE) {
+        uint8_t* at = v + (c >> 3) * kSub + (base + r0 + sub) * 128 + (c & 7) * 16;
+        uint32_t odd = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint4 w = *reinterpret_cast<const uint4*>(at + k * AT_ONCE * 128);
+            odd |= static_cast<uint32_t>(not_finite<BF>(w) && base + r0 + k * AT_ONCE + sub < live) << k;
+        }
+        if (!__any_sync(0xffffffffu, odd != 0) && base + r0 + 8 * AT_ONCE <= live) continue;
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t hit = __ballot_sync(0xffffffffu, (odd >> k) & 1);
+            const uint32_t row_mask = (1u << LANES) - 1u;
+            if (((hit >> (sub * LANES)) & row_mask) || base + r0 + k * AT_ONCE + sub >= live)
+                *reinterpret_cast<uint4*>(at + k * AT_ONCE * 128) = make_uint4(0, 0, 0, 0);
+            for (int q = 0; q < AT_ONCE; ++q) {
+                const int r = r0 + k * AT_ONCE + q;
+                if ((hit >> (q * LANES)) & row_mask) bad[r >> 5] |= 1u << (r & 31);
+            }
+        }
+    }
 }
 
 // The weight exp2((q . k) c - shift) of one key for one query row, worked out anew: for the few values that are not
