@@ -318,54 +318,59 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
             bar_arrive(rows_bar);
             wait_warp(rows_bar, syncs++ & 1);
         };
-        for (int i = 0;; ++i) {
-            Unit x;
-            if (!next_unit(x)) break;
-            if (x.nt > 0) {
-                // Query terms: a warp's 16 rows, eight rows' loads in flight, a row spread over the lanes. The scores
-                // that read the last unit's terms are done: every row thread has seen its last.
-                for (int r0 = 0; r0 < 16; r0 += 8) {
-                    float y[8][HD / 32];
-                    const int row0 = (warp - 4) * 16 + r0;
+        // Query terms of a unit: a warp's 16 rows, eight rows' loads in flight, a row spread over the lanes. The scores
+        // that read the last unit's terms are done: every row thread has seen its last.
+        auto stage_query = [&](const Unit& x) {
+            if (x.nt == 0) return;
+            for (int r0 = 0; r0 < 16; r0 += 8) {
+                float y[8][HD / 32];
+                const int row0 = (warp - 4) * 16 + r0;
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        const float* q = static_cast<const float*>(a.q) +
-                                         static_cast<long long>(x.s.q0 + x.tok + min(row0 + r, x.rows - 1)) * a.q_stride +
-                                         x.head * HD + lane * (HD / 32);
-                        if constexpr (HD == 128) {
-                            const float4 w = __ldg(reinterpret_cast<const float4*>(q));
-                            y[r][0] = w.x; y[r][1] = w.y; y[r][2] = w.z; y[r][3] = w.w;
-                        } else {
-                            const float2 w = __ldg(reinterpret_cast<const float2*>(q));
-                            y[r][0] = w.x; y[r][1] = w.y;
-                        }
-                    }
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        float top = 0.f;
-#pragma unroll
-                        for (int k = 0; k < HD / 32; ++k) top = fmaxf(top, fabsf(y[r][k]));
-                        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-                        // 2^bits lifts the row's largest value to [2^13, 2^14)
-                        const int bits = top > 0.f && top < __int_as_float(0x7F800000) ? min(13 - ilogbf(top), 126) : 0;
-                        const float up = ldexpf(1.f, bits);
-                        if (lane == 0) factor_s[row0 + r] = ldexpf(a.scale * 1.44269504088896341f, -bits);
-#pragma unroll
-                        for (int k = 0; k < HD / 32; k += 2) {
-                            uint32_t term[N];
-                            split<T, N>(y[r][k] * up, y[r][k + 1] * up, term);
-                            const int d = lane * (HD / 32) + k;  // dim
-#pragma unroll
-                            for (int t = 0; t < N; ++t)
-                                *reinterpret_cast<uint32_t*>(q_s + t * TILE + (d >> 6) * kSub + (row0 + r) * 128 +
-                                                             ((((d & 63) >> 3) ^ ((row0 + r) & 7)) << 4) + (d & 7) * 2) = term[t];
-                        }
+                for (int r = 0; r < 8; ++r) {
+                    const float* q = static_cast<const float*>(a.q) +
+                                     static_cast<long long>(x.s.q0 + x.tok + min(row0 + r, x.rows - 1)) * a.q_stride +
+                                     x.head * HD + lane * (HD / 32);
+                    if constexpr (HD == 128) {
+                        const float4 w = __ldg(reinterpret_cast<const float4*>(q));
+                        y[r][0] = w.x; y[r][1] = w.y; y[r][2] = w.z; y[r][3] = w.w;
+                    } else {
+                        const float2 w = __ldg(reinterpret_cast<const float2*>(q));
+                        y[r][0] = w.x; y[r][1] = w.y;
                     }
                 }
-                proxy_fence();
-                bar_arrive(q_full);
-                rows_sync();  // the rows' factors are there
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int k = 0; k < HD / 32; ++k) top = fmaxf(top, fabsf(y[r][k]));
+                    const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127;
+                    // 2^bits lifts the row's largest value to [2^13, 2^14); what is not finite stays so
+                    const int bits = min(13 - e, 126);
+                    const float up = __int_as_float((127 + bits) << 23);
+                    if (lane == 0) factor_s[row0 + r] = a.scale * 1.44269504088896341f * __int_as_float((127 - bits) << 23);
+                    uint32_t term[HD / 64][N];
+#pragma unroll
+                    for (int k = 0; k < HD / 64; ++k) split<T, N>(y[r][2 * k] * up, y[r][2 * k + 1] * up, term[k]);
+                    const int d = lane * (HD / 32);  // first dim
+#pragma unroll
+                    for (int t = 0; t < N; ++t) {
+                        uint8_t* at = q_s + t * TILE + (d >> 6) * kSub + (row0 + r) * 128 +
+                                      ((((d & 63) >> 3) ^ ((row0 + r) & 7)) << 4) + (d & 7) * 2;
+                        if constexpr (HD == 128) *reinterpret_cast<uint2*>(at) = make_uint2(term[0][t], term[HD / 64 - 1][t]);
+                        else *reinterpret_cast<uint32_t*>(at) = term[0][t];
+                    }
+                }
             }
+            proxy_fence();
+            bar_arrive(q_full);
+        };
+        Unit x;
+        bool have = next_unit(x);
+        if (have) {
+            stage_query(x);
+            rows_sync();  // the rows' factors are there
+        }
+        for (int i = 0; have && ok; ++i) {
             const float f = factor_s[row];
             const int limit = x.s.m - x.s.n + x.tok + row;  // the last key this row sees
             float ref = kNegInf, sum = 0.f, keep = 1.f, o[DIMS];
@@ -442,6 +447,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
                 if (j > 0) take_out();
                 keep = next_keep;
             }
+            // The next unit's query terms before this one's end: its first scores are made meanwhile.
+            Unit y;
+            const bool more = ok && next_unit(y);
+            if (more) stage_query(y);
             if (x.nt > 0 && ok) take_out();
             if (!ok) break;
             swap[0][half][row] = sum;
@@ -487,6 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
                 }
                 __syncwarp();
             }
+            have = more;
+            if (more) x = y;
         }
     }
     }
