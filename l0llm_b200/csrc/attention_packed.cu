@@ -190,22 +190,26 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         if (lane == 0) {
             proxy_fence();
             int e = 0, q_uses = 0;
-            int u = blockIdx.x < static_cast<unsigned>(total) ? static_cast<int>(blockIdx.x) : -1;
-            for (int i = 0; ok; ++i) {
-                const int slot = i % kUnitSlots;
-                if (!wait(read + 8 * slot, ((i / kUnitSlots) & 1) ^ 1)) break;
-                if (u < 0) {
-                    unit_s[slot].key_tiles = -1;
-                    bar_arrive(drawn + 8 * slot);
-                    break;
-                }
-                const Unit x = unit_at<PAIR>(a, pre, u);
+            int drawn_units = 0;
+            // Draws, works out and hands on the next unit: one ahead of the unit whose tiles are being fetched.
+            auto draw = [&]() {
+                Unit x;
+                unsigned u = blockIdx.x;
+                if (drawn_units > 0) u = atomicAdd(L.counters, 1u) + gridDim.x;
+                const int slot = drawn_units % kUnitSlots;
+                if (u < static_cast<unsigned>(total)) x = unit_at<PAIR>(a, pre, static_cast<int>(u));
+                else x.key_tiles = -1;
+                if (!wait(read + 8 * slot, ((drawn_units / kUnitSlots) & 1) ^ 1)) x.key_tiles = -1;
                 unit_s[slot] = x;
-                any_bad_s[i & 7] = 0;
+                any_bad_s[drawn_units & 7] = 0;
                 bar_arrive(drawn + 8 * slot);
-                const unsigned ahead = atomicAdd(L.counters, 1u) + gridDim.x;
-                u = ahead < static_cast<unsigned>(total) ? static_cast<int>(ahead) : -1;
-                if (x.key_tiles == 0) continue;
+                ++drawn_units;
+                return x;
+            };
+            Unit next = draw();
+            while (next.key_tiles >= 0 && ok) {
+                const Unit x = next;
+                if (x.key_tiles == 0) next = draw();
                 const int kvh = x.head[0] / (a.nh / a.nkv);
                 for (int k = 0; k < 2 * x.key_tiles; ++k, ++e) {  // K_0, Q, V_0, K_1, V_1, ...
                     const int st = e % kRing;
@@ -226,6 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                         for (int b = 0; b < BLOCKS; ++b)
                             tma_load(smem_addr(q_s) + t * TILE + b * kSub, &L.qmap, q_full, x.head[t] * HD + 64 * b, x.s.q0 + x.tok[t]);
                     }
+                    next = draw();
                 }
             }
             if (!ok) {  // no copy of this CTA's stays in flight behind it

@@ -186,21 +186,26 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
         if (lane == 0) {
             proxy_fence();
             int e = 0;
-            int u = blockIdx.x < static_cast<unsigned>(total) ? static_cast<int>(blockIdx.x) : -1;
-            for (int i = 0; ok; ++i) {
-                const int slot = i % kUnitSlots;
-                if (!wait(read + 8 * slot, ((i / kUnitSlots) & 1) ^ 1)) break;
-                if (u < 0) {
-                    unit_s[slot].nt = -1;
-                    bar_arrive(drawn + 8 * slot);
-                    break;
-                }
-                const Unit x = unit_at(a, pre, u);
+            int drawn_units = 0;
+            // Draws, works out and hands on the next unit: one ahead of the unit whose tiles are being fetched.
+            auto draw = [&]() {
+                Unit x;
+                unsigned u = blockIdx.x;
+                if (drawn_units > 0) u = atomicAdd(L.counters, 1u) + gridDim.x;
+                const int slot = drawn_units % kUnitSlots;
+                if (u < static_cast<unsigned>(total)) x = unit_at(a, pre, static_cast<int>(u));
+                else x.nt = -1;
+                if (!wait(read + 8 * slot, ((drawn_units / kUnitSlots) & 1) ^ 1)) x.nt = -1;
                 unit_s[slot] = x;
-                any_bad_s[i & 7] = 0;
+                any_bad_s[drawn_units & 7] = 0;
                 bar_arrive(drawn + 8 * slot);
-                const unsigned ahead = atomicAdd(L.counters, 1u) + gridDim.x;
-                u = ahead < static_cast<unsigned>(total) ? static_cast<int>(ahead) : -1;
+                ++drawn_units;
+                return x;
+            };
+            Unit next = draw();
+            while (next.nt >= 0 && ok) {
+                const Unit x = next;
+                if (x.nt == 0) next = draw();
                 const int kvh = x.head / (a.nh / a.nkv);
                 for (int k = 0; k < 2 * x.nt; ++k, ++e) {
                     const int st = e % R;
@@ -212,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
                     for (int b = 0; b < BLOCKS; ++b)
                         tma_load(smem_addr(kv_s) + st * TILE + b * kSub, is_v ? &L.vmap : &L.kmap, kv_full + 8 * st,
                                  kvh * HD + 64 * b, x.s.k0 + j * kRows);
+                    if (k == 0) next = draw();
                 }
             }
             if (!ok) {  // no copy of this CTA's stays in flight behind it
@@ -496,6 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
                 }
                 __syncwarp();
             }
+            rows_sync();  // every warp is done with its stage: the next unit's exchanges may take the place
             have = more;
             if (more) x = y;
         }
