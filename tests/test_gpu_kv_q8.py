@@ -269,6 +269,76 @@ def test_long_contexts(lz, device, suite, count, length, nh, nkv):
     c.dispose()
 
 
+def test_more_kv_heads_than_ctas(lz, device, suite):
+    # heads take turns: 200 KV heads on one team of warps a CTA
+    rng = np.random.default_rng(21)
+    c = Cache(lz, device, suite, 2, 3100, 200, 64, 64, rng, scale=0.01)
+    got, want, bound = attend(lz, device, suite, c, 200, [1, 1], [3100, 2900], "f32", starts=None)
+    assert_within(got, want, bound)
+    c.dispose()
+
+
+def test_as_many_sequences_as_a_call_takes(lz, device, suite):
+    rng = np.random.default_rng(22)
+    count, max_seq = 4096, 40
+    c = Cache(lz, device, suite, count, max_seq, 1, 128, 32)
+    n = rng.integers(0, 3, count)
+    n[100], pos = 30, np.zeros(count, int)
+    (k, v), (kv, vv) = rows_of(rng, int(n.sum()), 128, "f16")
+    c.store(k, v, "f16", n, pos)
+    c.store_model(kv, vv, n, pos)
+    c.check()
+    got, want, bound = attend(lz, device, suite, c, 2, n.tolist(), n.tolist(), "f32")
+    assert_within(got, want, bound)
+    rows = int(n.sum())
+    st, po = c.int_buffer(np.concatenate([[0], np.cumsum(n)])), c.int_buffer(pos)
+    out = [lz.SharedBuffer(device, lz.F32, rows * 128) for _ in range(2)]
+    suite.KvCacheQ8.Load(device, *c.buffers, *out, st, po, 1, 128, 32, max_seq, count, rows)
+    for w in range(2):
+        want = np.concatenate([so.values(c.codes[w][i, :m], c.scales[w][i], 32) for i, m in enumerate(n)])
+        np.testing.assert_array_equal(out[w].ToArray().reshape(rows, 128), want[:, 0].astype(np.float32))
+    for x in (st, po, *out):
+        x.Dispose()
+    c.dispose()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_query_that_is_not_finite_spoils_its_own_row(lz, device, suite, bad, dt):
+    rng = np.random.default_rng(23)
+    c = Cache(lz, device, suite, 2, 300, 2, 64, 32, rng, scale=0.01)
+    q = rng.standard_normal((3, 14, 64))
+    le, st = c.int_buffer([300, 77]), c.int_buffer([0, 2, 3])
+    got = []
+    for spoil in (False, True):
+        if spoil:
+            q[1, 4, 9] = bad
+        with lz.SharedBuffer.from_array(device, as_type(q, dt)[0], code(lz, dt)) as qb, \
+                lz.SharedBuffer(device, code(lz, dt), q.size) as ob:
+            suite.Attention.ExecuteQ8(device, qb, *c.buffers, ob, st, le, 64, 14, 2, 32, 300, 2, 3)
+            got.append(from_type(ob.ToArray(), dt).reshape(3, 14, 64))
+    assert not np.isfinite(got[1][1, 4]).any()
+    got[1][1, 4] = got[0][1, 4]
+    np.testing.assert_array_equal(got[0], got[1])
+    for x in (le, st):
+        x.Dispose()
+    c.dispose()
+
+
+def test_descending_starts_run_nothing(lz, device, suite):
+    rng = np.random.default_rng(24)
+    c = Cache(lz, device, suite, 3, 64, 1, 64, 32, rng, scale=0.01)
+    st, le = c.int_buffer([0, 6, 1, 6]), c.int_buffer([60, 60, 60])  # eleven rows out of six
+    status(lz, device)
+    with lz.SharedBuffer(device, lz.F32, 6 * 64) as qb, lz.SharedBuffer.from_array(device, np.full(6 * 64, 3, np.float32)) as ob:
+        suite.Attention.ExecuteQ8(device, qb, *c.buffers, ob, st, le, 64, 1, 1, 32, 64, 3, 6)
+        assert status(lz, device) & 2
+        assert np.all(ob.ToArray() == 3)
+    for x in (st, le):
+        x.Dispose()
+    c.dispose()
+
+
 def test_scales_that_differ_much(lz, device, suite):
     # a loud block beside quiet ones: their share of the output keeps its accuracy
     rng = np.random.default_rng(5)

@@ -140,6 +140,36 @@ def test_many_sequences(lz, device, suite, qt, kt):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("qt,kt", [("bf16", "bf16"), ("f32", "f16"), ("f32", "bf16")])
+def test_as_many_sequences_as_a_call_takes(lz, device, suite, qt, kt):
+    n = (np.arange(4096) % 3 == 1).astype(int).tolist()
+    n[7], n[4095] = 140, 3
+    c = Packed(lz, device, suite, 128, 1, 1, n, n, qt, kt)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+def test_no_keys_at_all(lz, device, suite, qt, kt):
+    c = Packed(lz, device, suite, 64, 2, 1, [5, 130], [0, 0], qt, kt)
+    assert not c.run().any()
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_query_that_is_not_finite_spoils_its_own_row(lz, device, suite, bad, qt, kt):
+    clean = Packed(lz, device, suite, 128, 4, 2, [140, 20], [200, 20], qt, kt)
+
+    def edit(q, k, v):
+        q[33, 128 + 7] = bad  # row 33, head 1
+
+    dirty = Packed(lz, device, suite, 128, 4, 2, [140, 20], [200, 20], qt, kt, edit=edit)
+    with np.errstate(all="ignore"):
+        got, want = dirty.run(), clean.run()
+    assert not np.isfinite(got[33, 1]).any()
+    got[33, 1] = want[33, 1]
+    np.testing.assert_array_equal(got, want)
+
+
 @pytest.mark.parametrize("qt,kt", TYPES)
 def test_large_scores_pick_one_key(lz, device, suite, qt, kt):
     def edit(q, k, v):
