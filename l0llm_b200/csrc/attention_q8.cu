@@ -72,8 +72,8 @@ struct Walk {
 
     __device__ __forceinline__ void sequence(int i, int& row0, int& n, int& len) const {
         const int s = a.starts ? __ldg(a.starts + i) : i, e = a.starts ? __ldg(a.starts + i + 1) : i + 1;
-        row0 = max(s, 0);
-        n = max(0, min(e, a.tokens) - row0);
+        row0 = clamp_start(s, a.tokens);
+        n = max(0, clamp_start(e, a.tokens) - row0);
         len = max(0, min(__ldg(a.lengths + i), a.max_seq));
     }
     __device__ __forceinline__ int column_groups(int n) const { return (n * (a.nh / a.nkv) + 8 * NT - 1) / (8 * NT); }
@@ -203,7 +203,8 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             int row0, n, len;
             walk.sequence(i, row0, n, len);
             if (blockIdx.x == 0 && (__ldg(a.lengths + i) != len ||
-                                    (a.starts && (__ldg(a.starts + i) < 0 || __ldg(a.starts + i + 1) > a.tokens))))
+                                    (a.starts && (__ldg(a.starts + i) < 0 || __ldg(a.starts + i + 1) > a.tokens ||
+                                                  __ldg(a.starts + i) > __ldg(a.starts + i + 1)))))
                 flag_bad_index(a.error);
             units += walk.units(n, len);
             items += walk.column_groups(n);

@@ -26,6 +26,14 @@ __device__ __forceinline__ int code_of_f64(double x, float scale) {
     return static_cast<int>(fmin(127.0, fmax(-127.0, rint(x / static_cast<double>(scale)))));
 }
 
+// Starts that ascend lie inside the buffer if the first and the last do; sequences wholly outside have no row that
+// would show it.
+__device__ __forceinline__ void check_ends(const KvQ8Params& p) {
+    if (!p.starts || blockIdx.x != 0 || threadIdx.x != 0) return;
+    const int first = p.starts[0], last = p.starts[p.count];
+    if (first != clamp_start(first, p.tokens) || last != clamp_start(last, p.tokens)) flag_bad_index(p.error);
+}
+
 template <typename T>
 __device__ __forceinline__ float2 pair_of(const uint32_t* w, int i) {  // values 2 i, 2 i + 1
     if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
@@ -76,6 +84,7 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
     const int row0 = tid / (HD / 8), col = tid % (HD / 8) * 8, step = blockDim.x / (HD / 8);
     pdl_wait();
     pdl_launch_dependents();
+    check_ends(p);
 
     const int t0 = range * rows_per_cta, t1 = min(p.tokens, t0 + rows_per_cta);
     int seq = p.starts ? block_find_sequence(p.starts, p.count, t0) : t0;
@@ -84,7 +93,7 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
         const int first = p.starts ? p.starts[seq] : seq, end_raw = p.starts ? p.starts[seq + 1] : seq + 1;
         if (first >= t1) break;
         const int pos = p.positions[seq];
-        const int end = min(end_raw, p.tokens);
+        const int end = clamp_start(end_raw, p.tokens);
         if (first < 0 || end_raw > p.tokens || pos < 0 || (end > first && pos > p.max_seq - (end - first))) {
             if (tid == 0) flag_bad_index(p.error);
             if (first < 0 || pos < 0 || pos >= p.max_seq) continue;
@@ -92,7 +101,7 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
         const int stop = min(end - first, p.max_seq - pos) + pos;  // past the sequence's last new slot
         // Leaders of this sequence in [t0, t1): its first row, then every row that opens a block.
         long long t = first;
-        if (t < t0) t = t0 + (-(pos + (t0 - first)) & (p.block - 1));
+        if (t < t0) t = t0 + static_cast<int>(-(static_cast<unsigned>(pos) + (t0 - first)) & (p.block - 1));
         while (t < min(end, t1) && pos + (t - first) < stop) {
             const int slot = static_cast<int>(pos + (t - first));
             const int blk = slot >> block_log, base = blk << block_log;
@@ -157,7 +166,7 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
                         q[2 * i + 1] = __float_as_uint(n1);
                         worst = fmaxf(fmaxf(worst, fabsf(res[2 * i])), fabsf(res[2 * i + 1]));
                     }
-                    // a branch of the warp: as predicated code this was a third of the kernel's instructions
+                    // next to a half, which is rare: a branch of the warp
                     if (__any_sync(0xffffffffu, worst >= half)) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
@@ -187,6 +196,7 @@ __global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p, int
     constexpr int VEC = 16 / sizeof(T);  // codes of a thread's step: 16 bytes out
     pdl_wait();
     pdl_launch_dependents();
+    check_ends(p);
     const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int kvd = p.nkv * p.hd, hd_log = p.hd == 128 ? 7 : 6, block_log = 31 - __clz(p.block);
     int t = warp * rows;
@@ -214,10 +224,11 @@ __global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p, int
             pos = __ldg(p.positions + seq);
         }
         if (t < first) continue;
-        const bool fits = pos >= 0 && pos < p.max_seq - (t - first);
+        const long long nth = static_cast<long long>(t) - first;  // a start may be any number
+        const bool fits = pos >= 0 && pos + nth < p.max_seq;
         if (lane == 0 && (!fits || first < 0 || end > p.tokens)) flag_bad_index(p.error);
         if (!fits) continue;
-        const int slot = pos + (t - first);
+        const int slot = pos + static_cast<int>(nth);
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             const int8_t* src = (which ? p.vc : p.kc) + (static_cast<long long>(seq) * p.max_seq + slot) * kvd;

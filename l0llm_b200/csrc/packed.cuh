@@ -10,6 +10,9 @@ __device__ __forceinline__ void flag_bad_index(int* error) {
     if (error) atomicOr(error, 2);
 }
 
+// A start read on the device, kept within [0, rows]: differences of two of them cannot overflow.
+__device__ __forceinline__ int clamp_start(int start, int rows) { return max(0, min(start, rows)); }
+
 // Index of the last of starts[0, count) that is <= t, -1 if none: the sequence of packed row t when
 // t < starts[index + 1] (an empty sequence shares its start with the next and is passed over). All threads
 // of the CTA call it together and get the same answer; every start is read at once, so the latency is one

@@ -18,10 +18,10 @@ struct PackedSeq {
 
 __device__ __forceinline__ PackedSeq packed_seq(const PackedAttnParams& a, int i) {
     PackedSeq s;
-    s.q0 = max(__ldg(a.q_starts + i), 0);
-    s.n = max(0, min(__ldg(a.q_starts + i + 1), a.tokens) - s.q0);
-    s.k0 = max(0, min(__ldg(a.kv_starts + i), a.kv_tokens));
-    s.m = max(0, min(__ldg(a.kv_starts + i + 1), a.kv_tokens) - s.k0);
+    s.q0 = clamp_start(__ldg(a.q_starts + i), a.tokens);
+    s.n = max(0, clamp_start(__ldg(a.q_starts + i + 1), a.tokens) - s.q0);
+    s.k0 = clamp_start(__ldg(a.kv_starts + i), a.kv_tokens);
+    s.m = max(0, clamp_start(__ldg(a.kv_starts + i + 1), a.kv_tokens) - s.k0);
     return s;
 }
 

@@ -7,7 +7,7 @@ import ctypes as C
 import numpy as np
 import pytest
 import seq_oracle as so
-from test_gpu_packed import UNIT, as_type, code, from_type, status
+from test_gpu_packed import I32_MAX, I32_MIN, UNIT, as_type, code, from_type, status
 
 pytestmark = pytest.mark.gpu
 
@@ -191,6 +191,29 @@ def test_load_outside_the_cache(lz, device, suite):
         np.testing.assert_array_equal(got[:5], so.values(c.codes[w][0], c.scales[w][0], 32)[35:40, 0].astype(np.float32))
     for x in (st, po, *out):
         x.Dispose()
+    c.dispose()
+
+
+@pytest.mark.parametrize("starts", [[I32_MAX, I32_MIN], [I32_MIN, 6], [I32_MIN + 3, 6], [I32_MIN, I32_MIN], [7, 9]])
+def test_starts_far_outside(lz, device, suite, starts):
+    # differences that overflow, rows behind the buffer: no row that an op could serve, so all buffers stay as they are
+    rng = np.random.default_rng(33)
+    c = Cache(lz, device, suite, 1, 4, 1, 64, 32, rng)
+    st, po = c.int_buffer(starts), c.int_buffer([0])
+    x = [lz.SharedBuffer.from_array(device, np.full(6 * 64, 3, np.float32)) for _ in range(2)]
+    status(lz, device)
+    suite.KvCacheQ8.Load(device, *c.buffers, *x, st, po, 1, 64, 32, 4, 1, 6)
+    assert status(lz, device) == 2
+    suite.KvCacheQ8.Store(device, *x, *c.buffers, st, po, 1, 64, 32, 4, 1, 6)
+    assert status(lz, device) == 2
+    c.check()
+    if starts[1] != 6:
+        suite.Attention.ExecuteQ8(device, x[0], *c.buffers, x[1], st, po, 64, 1, 1, 32, 4, 1, 6)
+        assert status(lz, device) == 2
+    for b in x:
+        assert np.all(b.ToArray() == 3)
+    for b in (st, po, *x):
+        b.Dispose()
     c.dispose()
 
 

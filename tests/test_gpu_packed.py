@@ -10,6 +10,7 @@ import seq_oracle as so
 
 pytestmark = pytest.mark.gpu
 
+I32_MIN, I32_MAX = -2 ** 31, 2 ** 31 - 1
 UNIT = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}  # half a step
 # f32 queries: probabilities as sums of 16-bit terms, off by 2^-21 at most; 16-bit ones rounded to their type
 UNIT_P = {"f32": 2.0 ** -21, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
@@ -298,6 +299,23 @@ def test_starts_outside_the_buffers(lz, device, suite, q_starts, kv_starts, qt, 
     c.call(b)
     c.check(c.read(b))
     assert status(lz, device) == 0
+    for x in b:
+        x.Dispose()
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("q_starts,kv_starts,want", [([I32_MAX, I32_MIN], [0, 50], 7.0), ([0, 40], [1, I32_MIN], 0.0),
+                                                     ([0, 40], [I32_MAX, I32_MIN], 0.0), ([I32_MIN, I32_MIN], [0, 50], 7.0)])
+def test_starts_whose_differences_overflow(lz, device, suite, q_starts, kv_starts, want, qt, kt):
+    # no rows at all, or rows without keys
+    c = Packed(lz, device, suite, 128, 4, 2, [40], [50], qt, kt)
+    b = c.buffers()
+    status(lz, device)
+    b[4].Write(np.array(q_starts, np.int32))
+    b[5].Write(np.array(kv_starts, np.int32))
+    c.call(b)
+    assert status(lz, device) == 2
+    np.testing.assert_array_equal(c.read(b), want)
     for x in b:
         x.Dispose()
 
