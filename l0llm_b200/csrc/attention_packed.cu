@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                 if (!wait_warp(o_full + 8 * t, o_uses++ & 1)) break;
                 tc_after();
             }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            // A row without keys gives zeros; one whose every score is -inf has no weights, and 0 / 0 says so.
+            const float inv = limit < 0 ? 0.f : 1.f / sum;
             const bool any_bad = nt > 0 && *reinterpret_cast<volatile int*>(&any_bad_s[i & 7]) != 0;
             T* out = static_cast<T*>(a.out) + static_cast<long long>(x.s.q0 + x.tok[t] + (warp & 3) * 32) * a.out_stride + x.head[t] * HD;
 #pragma unroll 1

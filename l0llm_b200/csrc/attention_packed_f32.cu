@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
             if (!ok) break;
             swap[0][half][row] = sum;
             rows_sync();
-            const float all = swap[0][0][row] + swap[0][1][row], inv = all == 0.f ? 0.f : 1.f / all;
+            const float all = swap[0][0][row] + swap[0][1][row], inv = limit < 0 ? 0.f : 1.f / all;
             rows_sync();  // the sums are read: their place is the epilogue's
             if (!ok) break;
             const bool any_bad = x.nt > 0 && *reinterpret_cast<volatile int*>(&any_bad_s[i & 7]) != 0;

@@ -172,6 +172,25 @@ def test_a_query_that_is_not_finite_spoils_its_own_row(lz, device, suite, bad, q
 
 
 @pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("hd,m", [(128, 300), (64, 60)])
+def test_a_row_whose_scores_are_all_minus_infinity(lz, device, suite, hd, m, qt, kt):
+    # it sees keys, so it is not a row of zeros: exp(-inf - -inf) has no value
+    def edit(q, k, v):
+        q[3, :hd] = 0
+        q[3, 0] = np.inf
+        k[:, 0] = -1
+
+    c = Packed(lz, device, suite, hd, 2, 1, [50], [m], qt, kt, edit=edit)
+    b = c.buffers()
+    c.call(b)
+    got = c.read(b)
+    assert np.all(np.isnan(got[3, 0])) and np.all(np.isfinite(got[3, 1]))
+    assert np.all(np.isfinite(np.delete(got, 3, 0)))
+    for x in b:
+        x.Dispose()
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
 def test_large_scores_pick_one_key(lz, device, suite, qt, kt):
     def edit(q, k, v):
         q *= 30.0
