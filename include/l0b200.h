@@ -277,11 +277,12 @@ L0B_API l0b_status l0b_attention_execute_prefill(l0b_suite* s, l0b_device* d, l0
  *
  * q [tokens, nH * hd] and out: f32, or the type of k and v; k, v [kv_tokens, nKv * hd]: f16 or bf16 (the types a
  * KvCacheStore writes; stored at position 0 the rows of several prompts are such a packed buffer). Row strides
- * in elements (<= 0: packed rows), so q, k and v may be column views of one stacked projection. k, v and 16-bit q
- * rows start on 16 bytes (base and stride). hd 64 or 128; count <= 4096. out must not overlap the inputs.
+ * in elements (<= 0: packed rows), so q, k and v may be column views of one stacked projection. Rows of q, k, v and
+ * out start on 16 bytes (base and stride). hd 64 or 128; count <= 4096. out must not overlap the inputs.
  * f32 queries keep about f32 accuracy (queries and probabilities enter the MMA as sums of 16-bit terms); 16-bit
  * queries meet probabilities rounded to their own type, summed in f32. A masked key's or value's contents never
- * reach a row, whatever they are. */
+ * reach a row, whatever they are; a row that does see a key or value that is not finite need not be finite.
+ * Starts that descend, so that sequences share query rows, run nothing and set the error status. */
 L0B_API l0b_status l0b_attention_execute_packed(l0b_suite* s, l0b_device* d, l0b_buffer* q, l0b_buffer* k,
                                                 l0b_buffer* v, l0b_buffer* out, l0b_buffer* q_starts,
                                                 l0b_buffer* kv_starts, int32_t head_dim, int32_t n_heads,
@@ -296,7 +297,8 @@ L0B_API l0b_status l0b_attention_execute_packed(l0b_suite* s, l0b_device* d, l0b
  * call is row i of these buffers (l0b_buffer_view names a run of rows). All zero (as allocated) is a valid empty
  * cache. starts: i32 [count + 1], the packed rows of each sequence as in l0b_attention_execute_packed; NULL: one
  * row a sequence (tokens == count). positions / lengths: i32 [count]. All are read on the device, so a recorded
- * command list follows their contents; starts ascend. hd 64 or 128; count <= 4096.
+ * command list follows their contents; starts ascend. hd 64 or 128; count <= 4096. Rows of k, v, q, out and of the
+ * cache start on 16 bytes (base and stride).
  *
  * Store: rows of k / v [tokens, nKv * hd] (f32, f16 or bf16, row strides as above) go to slots positions[i],
  * positions[i] + 1, ... The scale of a block is f32(max|x| / 127) over its new rows and the codes are

@@ -146,11 +146,11 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
             if (kept > 0) scale = __uint_as_float(max(__float_as_uint(old) & 0x7FFFFFFFu, __float_as_uint(scale)));
             const bool fine = scale > 0.f && scale < __int_as_float(0x7F800000);
             int8_t* dst = cache + (static_cast<long long>(seq) * p.max_seq + base) * kvd;
-            if (kept > 0 && __float_as_uint(scale) != __float_as_uint(old))
-                rescale_kept(dst, kvd, HD == 128 ? 7 : 6, kept, old, scale, fine);
             dst += static_cast<long long>(kept) * kvd;
             if (fine && scale > 1e-36f) {  // the reciprocal and every residual next to a half are normal numbers
-                const float inv = 1.f / scale, half = 0.5f * scale;
+                const float half = 0.5f * scale, inv1 = 1.f / scale;
+                const float2 inv = make_float2(inv1, inv1), minus = make_float2(-scale, -scale);
+                const float2 magic = make_float2(12582912.f, 12582912.f), unmagic = make_float2(-12582912.f, -12582912.f);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     uint32_t q[8];
@@ -159,11 +159,11 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
                     for (int i = 0; i < 4; ++i) {
                         // 1.5 2^23 + the nearest integer: its low byte is the code
                         const float2 x = pair_of<T>(w[g], i);
-                        const float n0 = fmaf(x.x, inv, 12582912.f), n1 = fmaf(x.y, inv, 12582912.f);
-                        res[2 * i] = fmaf(12582912.f - n0, scale, x.x);
-                        res[2 * i + 1] = fmaf(12582912.f - n1, scale, x.y);
-                        q[2 * i] = __float_as_uint(n0);
-                        q[2 * i + 1] = __float_as_uint(n1);
+                        const float2 n = ffma2(x, inv, magic), r = ffma2(fadd2(n, unmagic), minus, x);
+                        res[2 * i] = r.x;
+                        res[2 * i + 1] = r.y;
+                        q[2 * i] = __float_as_uint(n.x);
+                        q[2 * i + 1] = __float_as_uint(n.y);
                         worst = fmaxf(fmaxf(worst, fabsf(res[2 * i])), fabsf(res[2 * i + 1]));
                     }
                     // next to a half, which is rare: a branch of the warp
@@ -183,6 +183,8 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
             } else {
                 store_slowly<T, HD>(src + t * stride, stride, dst, kvd, n, scale, fine);
             }
+            if (kept > 0 && __float_as_uint(scale) != __float_as_uint(old))  // last: nothing else is held over the call
+                rescale_kept(dst - static_cast<long long>(kept) * kvd, kvd, HD == 128 ? 7 : 6, kept, old, scale, fine);
             if (tid == 0) *sp = scale;
             t += n;
         }
