@@ -4,7 +4,7 @@
 // sequence that land in one block of slots; the row that opens it is its leader), for one KV head of K or V.
 // Every new value of a piece stays in registers between the two things done with it: the largest magnitude
 // (bits of |x| compared as integers, so an infinity or a NaN wins and the scale shows it) and the codes. So
-// the rows are read once and the codes written once. 22,200 bf16 rows of 8 heads of 128 take 41 us, 3.3 TB/s: a piece
+// the rows are read once and the codes written once. 22,200 bf16 rows of 8 heads of 128 take 38 us, 3.5 TB/s: a piece
 // is a chain of a fetch, a maximum over the CTA and a write, and two CTAs an SM (64 registers) hide some of it; three of
 // 40 registers spill and took 7% longer.
 //
@@ -193,75 +193,70 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
     }
 }
 
-// Load. A warp takes a run of packed rows, K and V of each: 128 or 256 codes a step into 512 contiguous bytes. Bound
-// by HBM: 38,270 rows of 8 heads of 128 as f16 take 46 us, 5.1 TB/s.
+// Load. A warp takes one packed row, K and V of it: 128 or 256 codes a step into 512 contiguous bytes. Bound by HBM:
+// 76,545 rows of 8 heads of 128 as f16 take 86 us, 5.5 TB/s. (Warps that took a run of rows, to find their sequence once,
+// took 87, and 194 instead of 156 for 4000 short sequences; finding one of 4096 takes three reads.)
 template <typename T>
-__global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p, int rows) {
+__global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p) {
     constexpr int VEC = 16 / sizeof(T);  // codes of a thread's step: 16 bytes out
     pdl_wait();
     pdl_launch_dependents();
     if (blockIdx.x == gridDim.x - 1) return check_ends(p);
-    const int lane = threadIdx.x & 31, warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int kvd = p.nkv * p.hd, hd_log = p.hd == 128 ? 7 : 6, block_log = 31 - __clz(p.block);
-    int t = warp * rows;
-    const int t1 = min(p.tokens, t + rows);
-    if (t >= t1) return;
-    int seq = t, first = t, end = t, pos = 0;
-    if (p.starts) {  // the last sequence that starts at or before the run
-        seq = -1;
-        for (int i = lane; __any_sync(0xffffffffu, i < p.count); i += 32)
-            seq += __popc(__ballot_sync(0xffffffffu, i < p.count && __ldg(p.starts + i) <= t));
-        first = end = INT32_MIN;
-        --seq;
-    }
-    for (; t < t1; ++t) {
-        if (!p.starts) {
-            seq = first = t;
-            end = t + 1;
-            pos = __ldg(p.positions + t);
-        } else if (t >= end) {  // on to the sequence of this row
-            do ++seq;
-            while (seq < p.count && (seq < 0 || __ldg(p.starts + seq + 1) <= t));
-            if (seq >= p.count) return;
-            first = __ldg(p.starts + seq);
-            end = __ldg(p.starts + seq + 1);
-            pos = __ldg(p.positions + seq);
+    if (t >= p.tokens) return;
+    int seq = t, first = t;
+    if (p.starts) {  // the last sequence that starts at or before the row: each step looks at 32 of those left
+        int before = 0, left = p.count;
+        while (left > 0) {
+            const int step = (left + 31) / 32, i = before + (lane + 1) * step - 1;
+            const int n = step * __popc(__ballot_sync(0xffffffffu, i < before + left && __ldg(p.starts + i) <= t));
+            before += n;
+            left = min(left - n, step - 1);
         }
-        if (t < first) continue;
-        const long long nth = static_cast<long long>(t) - first;  // a start may be any number
-        const bool fits = pos >= 0 && pos + nth < p.max_seq;
-        if (lane == 0 && (!fits || first < 0 || end > p.tokens)) flag_bad_index(p.error);
-        if (!fits) continue;
-        const int slot = pos + static_cast<int>(nth);
+        seq = before - 1;
+        if (seq < 0) return;
+        first = __ldg(p.starts + seq);
+        const int end = __ldg(p.starts + seq + 1);
+        if (lane == 0 && (first < 0 || end > p.tokens)) flag_bad_index(p.error);
+        if (t >= end) return;
+    }
+    const int pos = __ldg(p.positions + seq);
+    const long long nth = static_cast<long long>(t) - first;  // a start may be any number
+    if (pos < 0 || pos + nth >= p.max_seq) {
+        if (lane == 0) flag_bad_index(p.error);
+        return;
+    }
+    const int slot = pos + static_cast<int>(nth);
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const int8_t* src = (which ? p.vc : p.kc) + (static_cast<long long>(seq) * p.max_seq + slot) * kvd;
-            const float* scales = (which ? p.vs : p.ks) + (static_cast<long long>(seq) * p.blocks + (slot >> block_log)) * p.nkv;
-            T* dst = static_cast<T*>(const_cast<void*>(which ? p.v : p.k)) + t * (which ? p.v_stride : p.k_stride);
+    for (int which = 0; which < 2; ++which) {
+        const int8_t* src = (which ? p.vc : p.kc) + (static_cast<long long>(seq) * p.max_seq + slot) * kvd;
+        const float* scales = (which ? p.vs : p.ks) + (static_cast<long long>(seq) * p.blocks + (slot >> block_log)) * p.nkv;
+        T* dst = static_cast<T*>(const_cast<void*>(which ? p.v : p.k)) + t * (which ? p.v_stride : p.k_stride);
 #pragma unroll 4
-            for (int c = lane * VEC; c < kvd; c += 32 * VEC) {
-                const float scale = __ldg(scales + (c >> hd_log));
-                float v[8];
-                uint32_t w[2];
-                if constexpr (VEC == 4) {
-                    w[0] = __ldg(reinterpret_cast<const unsigned*>(src + c));
-                } else {
-                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(src + c));
-                    w[0] = u.x;
-                    w[1] = u.y;
-                }
-#pragma unroll
-                for (int j = 0; j < VEC / 4; ++j) {
-                    float2 a, b;
-                    dequant_i8x4(w[j], a, b);
-                    v[4 * j] = a.x * scale;
-                    v[4 * j + 1] = a.y * scale;
-                    v[4 * j + 2] = b.x * scale;
-                    v[4 * j + 3] = b.y * scale;
-                }
-                if constexpr (VEC == 4) *reinterpret_cast<float4*>(dst + c) = make_float4(v[0], v[1], v[2], v[3]);
-                else store8(dst + c, v);
+        for (int c = lane * VEC; c < kvd; c += 32 * VEC) {
+            const float scale = __ldg(scales + (c >> hd_log));
+            float v[8];
+            uint32_t w[2];
+            if constexpr (VEC == 4) {
+                w[0] = __ldg(reinterpret_cast<const unsigned*>(src + c));
+            } else {
+                const uint2 u = __ldg(reinterpret_cast<const uint2*>(src + c));
+                w[0] = u.x;
+                w[1] = u.y;
             }
+#pragma unroll
+            for (int j = 0; j < VEC / 4; ++j) {
+                float2 a, b;
+                dequant_i8x4(w[j], a, b);
+                v[4 * j] = a.x * scale;
+                v[4 * j + 1] = a.y * scale;
+                v[4 * j + 2] = b.x * scale;
+                v[4 * j + 3] = b.y * scale;
+            }
+            // f32 rows go past the L2: 22,167 rows stored and read back took 78.5 us, now 70.7. 16-bit ones would lose 1%.
+            if constexpr (VEC == 4) __stcs(reinterpret_cast<float4*>(dst + c), make_float4(v[0], v[1], v[2], v[3]));
+            else store8(dst + c, v);
         }
     }
 }
@@ -283,9 +278,7 @@ l0b_status store_as(l0b_device* d, const KvQ8Params& p) {
 
 template <typename T>
 l0b_status load_as(l0b_device* d, const KvQ8Params& p) {
-    // Rows a warp: one, until 64 warps an SM have more than that.
-    const int rows = (p.tokens + 64 * d->sm_count - 1) / (64 * d->sm_count);
-    return d->launch(kv_q8_load_kernel<T>, dim3((p.tokens + 8 * rows - 1) / (8 * rows) + 1), dim3(256), 0, p, rows);
+    return d->launch(kv_q8_load_kernel<T>, dim3((p.tokens + 7) / 8 + 1), dim3(256), 0, p);
 }
 
 }  // namespace
