@@ -177,6 +177,30 @@ def test_load_matches_the_definition(lz, device, suite, hd, nkv, block, dt):
     c.dispose()
 
 
+@pytest.mark.parametrize("count", [1, 31, 32, 33, 64, 65, 1023, 1024, 1025])
+def test_load_of_many_sequences(lz, device, suite, count):
+    # empty ones among them, at both ends too, and rows in front of the first and behind the last
+    rng = np.random.default_rng(count)
+    c = Cache(lz, device, suite, count, 8, 1, 64, 32, rng)
+    n, pos = rng.integers(0, 4, count), rng.integers(0, 5, count)
+    n[0] = n[-1] = 0
+    n[count // 2] = 4
+    rows = int(n.sum()) + 5
+    st, po = c.int_buffer(np.concatenate([[0], np.cumsum(n)]) + 3), c.int_buffer(pos)
+    out = [lz.SharedBuffer.from_array(device, np.full(rows * 64, 9, np.float32)) for _ in range(2)]
+    status(lz, device)
+    suite.KvCacheQ8.Load(device, *c.buffers, *out, st, po, 1, 64, 32, 8, count, rows)
+    assert status(lz, device) == 0
+    for w in range(2):
+        got = out[w].ToArray().reshape(rows, 64)
+        assert np.all(got[:3] == 9) and np.all(got[rows - 2:] == 9)
+        want = np.concatenate([so.values(c.codes[w][i], c.scales[w][i], 32)[p:p + m] for i, (m, p) in enumerate(zip(n, pos))])
+        np.testing.assert_array_equal(got[3:rows - 2], want[:, 0].astype(np.float32))
+    for x in (st, po, *out):
+        x.Dispose()
+    c.dispose()
+
+
 def test_load_outside_the_cache(lz, device, suite):
     rng = np.random.default_rng(3)
     c = Cache(lz, device, suite, 2, 40, 1, 64, 32, rng)
