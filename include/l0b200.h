@@ -282,7 +282,8 @@ L0B_API l0b_status l0b_attention_execute_prefill(l0b_suite* s, l0b_device* d, l0
  * f32 queries keep about f32 accuracy (queries and probabilities enter the MMA as sums of 16-bit terms); 16-bit
  * queries meet probabilities rounded to their own type, summed in f32. A masked key's or value's contents never
  * reach a row, whatever they are; a row that does see a key or value that is not finite need not be finite.
- * Starts that descend, so that sequences share query rows, run nothing and set the error status. */
+ * Query starts that descend anywhere run nothing and set the error status; a sequence whose key starts descend has no
+ * keys, and sets it too. */
 L0B_API l0b_status l0b_attention_execute_packed(l0b_suite* s, l0b_device* d, l0b_buffer* q, l0b_buffer* k,
                                                 l0b_buffer* v, l0b_buffer* out, l0b_buffer* q_starts,
                                                 l0b_buffer* kv_starts, int32_t head_dim, int32_t n_heads,
@@ -322,8 +323,9 @@ L0B_API l0b_status l0b_kv_cache_q8_load(l0b_suite* s, l0b_device* d, l0b_buffer*
 /* Attention.Execute over the int8 cache for `count` sequences at once: sequence i holds lengths[i] slots, the last
  * of them the positions of its n query rows (one, or a few drafted tokens), and query t attends to slots
  * [0, lengths[i] - n + t] (none: zeros). q [tokens, nH * hd] and out: f32, f16 or bf16, one type; row strides in
- * elements (<= 0: packed rows). Products and sums keep about f32 accuracy against the cache's values. One launch
- * for any mix of lengths. Long blocks of queries are better served by Load and l0b_attention_execute_packed. */
+ * elements (<= 0: packed rows). Products and sums keep about f32 accuracy against the cache's values. Starts that
+ * descend anywhere run nothing and set the error status. One launch for any mix of lengths. Long blocks of queries are
+ * better served by Load and l0b_attention_execute_packed. */
 L0B_API l0b_status l0b_attention_execute_q8(l0b_suite* s, l0b_device* d, l0b_buffer* q, l0b_buffer* kc,
                                             l0b_buffer* vc, l0b_buffer* k_scales, l0b_buffer* v_scales,
                                             l0b_buffer* out, l0b_buffer* starts, l0b_buffer* lengths,

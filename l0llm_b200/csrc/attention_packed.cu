@@ -113,7 +113,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     __shared__ __align__(8) uint64_t bars[2 + 2 * kRing + 5 * 2 + kRing + 2 * kUnitSlots];
     __shared__ Unit unit_s[kUnitSlots];
     __shared__ int scan_s[kThreads / 32];
-    __shared__ unsigned long long rows_s;
     // Value rows that are not finite: [unit & 7][cut tile & 3]. The roles are at most kUnitSlots units apart.
     __shared__ uint32_t bad_s[8][4][4];
     __shared__ int any_bad_s[8];
@@ -145,7 +144,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
             bar_init(read + 8 * i, 11);  // MMA thread, two guard warps, eight softmax warps
         }
         bar_init_fence();
-        rows_s = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.qmap)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.kmap)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.vmap)) : "memory");
@@ -161,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     tc_after();
     const uint32_t tmem = tmem_s;
 
-    const bool fine = packed_scan(a, pre, scan_s, &rows_s, [&](int n) { return units_of<PAIR>(a, n); });
+    const bool fine = packed_scan(a, pre, scan_s, [&](int n) { return units_of<PAIR>(a, n); });
     const int total = pre[a.count];
     bool ok = true;  // false once a bounded wait gave up: the role stops
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -185,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     };
 
     // The launch's 168 registers a thread are dealt anew: 88 for the first warpgroup, 208 for the softmax threads.
-    // Starts that name rows more than once: nothing runs.
+    // Query starts that descend: nothing runs.
     if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (!fine) {

@@ -112,7 +112,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
     __shared__ __align__(8) uint64_t bars[1 + 3 * R + 2 * 2 + 3 + 2 * kUnitSlots];
     __shared__ Unit unit_s[kUnitSlots];
     __shared__ int scan_s[kThreads / 32], any_bad_s[8];
-    __shared__ unsigned long long rows_s;
     __shared__ uint32_t bad_s[8][2][4];  // [unit & 7][cut tile]: value rows that are not finite
     __shared__ float factor_s[kRows];
     __shared__ uint32_t tmem_s;
@@ -141,7 +140,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
             bar_init(read + 8 * i, 11);  // the MMA warp, two guard warps, eight row warps
         }
         bar_init_fence();
-        rows_s = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.kmap)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.vmap)) : "memory");
     }
@@ -157,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
     // Columns: scores and weight terms 0 and 1 of even and odd tiles, O, third terms of even and odd tiles.
     const uint32_t tmem = tmem_s, o_col = tmem + 2 * kRows, p2_col = tmem + 3 * kRows;
 
-    const bool fine = packed_scan(a, pre, scan_s, &rows_s, [&](int n) { return units_of(a, n); });
+    const bool fine = packed_scan(a, pre, scan_s, [&](int n) { return units_of(a, n); });
     const int total = pre[a.count];
     bool ok = true;  // false once a bounded wait gave up: the role stops
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -180,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
     };
 
     // The launch's 168 registers a thread are dealt anew: 88 for the first warpgroup, 208 for the row threads.
-    // Starts that name rows more than once: nothing runs.
+    // Query starts that descend: nothing runs.
     if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (!fine) {

@@ -179,7 +179,6 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     __shared__ __align__(8) uint64_t bars[W * kStages * 2];  // keys, values of each stage
     __shared__ float ml_s[W][COLS][2];
     __shared__ int scan_s[W][2];
-    __shared__ unsigned long long rows_s;
     __shared__ unsigned last_s[W];
     const AttnQ8Params& a = L.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -188,7 +187,6 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     if (threadIdx.x == 0) {
         for (int i = 0; i < W * kStages * 2; ++i) bar_init(smem_addr(&bars[i]), 1);
         bar_init_fence();
-        rows_s = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.kmap)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.vmap)) : "memory");
     }
@@ -199,17 +197,16 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     {
         const int per = (a.count + W * 32 - 1) / (W * 32), i0 = threadIdx.x * per, i1 = min(a.count, i0 + per);
         int units = 0, items = 0;
-        long long rows = 0;
+        bool descends = false;  // sequences could then share rows of out, which no order of writing settles
         for (int i = i0; i < i1; ++i) {
             int row0, n, len;
             walk.sequence(i, row0, n, len);
-            if (blockIdx.x == 0 && (__ldg(a.lengths + i) != len ||
-                                    (a.starts && (__ldg(a.starts + i) < 0 || __ldg(a.starts + i + 1) > a.tokens ||
-                                                  __ldg(a.starts + i) > __ldg(a.starts + i + 1)))))
+            descends |= a.starts && __ldg(a.starts + i) > __ldg(a.starts + i + 1);
+            if (blockIdx.x == 0 && (descends || __ldg(a.lengths + i) != len ||
+                                    (a.starts && (__ldg(a.starts + i) < 0 || __ldg(a.starts + i + 1) > a.tokens))))
                 flag_bad_index(a.error);
             units += walk.units(n, len);
             items += walk.column_groups(n);
-            rows += n;
         }
         int sum = units;
 #pragma unroll
@@ -223,12 +220,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             scan_s[warp][0] = sum;
             scan_s[warp][1] = items;
         }
-        if (rows) atomicAdd(&rows_s, static_cast<unsigned long long>(rows));
-        __syncthreads();
-        if (rows_s > static_cast<unsigned long long>(a.tokens)) {  // starts that descend name rows more than once
-            if (threadIdx.x == 0) flag_bad_index(a.error);
-            return;
-        }
+        if (__syncthreads_or(descends)) return;  // nothing runs
         int before = sum - units;
         for (int w = 0; w < warp; ++w) before += scan_s[w][0];
         for (int i = i0; i < i1; ++i) {

@@ -26,22 +26,18 @@ __device__ __forceinline__ PackedSeq packed_seq(const PackedAttnParams& a, int i
 }
 
 // pre[i] = the sum of units(n) over the sequences before i, pre[count] the total, by the whole CTA. False (and the
-// error flag) when the sequences together have more rows than the buffer, which ascending starts never have.
+// error flag) where the query starts descend: sequences could then share rows of out, which no order of writing settles.
 template <typename F>
-__device__ __forceinline__ bool packed_scan(const PackedAttnParams& a, int* pre, int* warp_sums, unsigned long long* rows_s,
-                                            F units) {
+__device__ __forceinline__ bool packed_scan(const PackedAttnParams& a, int* pre, int* warp_sums, F units) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int per = (a.count + blockDim.x - 1) / blockDim.x, i0 = threadIdx.x * per, i1 = min(a.count, i0 + per);
     int mine = 0;
-    long long rows = 0;
-    bool bad = false;
+    bool bad = false, descends = false;
     for (int i = i0; i < i1; ++i) {
-        const PackedSeq s = packed_seq(a, i);
-        mine += units(s.n);
-        rows += s.n;
-        bad |= __ldg(a.q_starts + i) < 0 || __ldg(a.q_starts + i + 1) > a.tokens || __ldg(a.kv_starts + i) < 0 ||
-               __ldg(a.kv_starts + i + 1) > a.kv_tokens || __ldg(a.q_starts + i) > __ldg(a.q_starts + i + 1) ||
-               __ldg(a.kv_starts + i) > __ldg(a.kv_starts + i + 1);
+        mine += units(packed_seq(a, i).n);
+        descends |= __ldg(a.q_starts + i) > __ldg(a.q_starts + i + 1);
+        bad |= descends || __ldg(a.q_starts + i) < 0 || __ldg(a.q_starts + i + 1) > a.tokens || __ldg(a.kv_starts + i) < 0 ||
+               __ldg(a.kv_starts + i + 1) > a.kv_tokens || __ldg(a.kv_starts + i) > __ldg(a.kv_starts + i + 1);
     }
     if (bad && blockIdx.x == 0) flag_bad_index(a.error);
     int sum = mine;
@@ -51,10 +47,7 @@ __device__ __forceinline__ bool packed_scan(const PackedAttnParams& a, int* pre,
         if (lane >= o) sum += up;
     }
     if (lane == 31) warp_sums[warp] = sum;
-    if (rows) atomicAdd(rows_s, static_cast<unsigned long long>(rows));
-    __syncthreads();
-    const bool fine = *rows_s <= static_cast<unsigned long long>(a.tokens);
-    if (!fine && threadIdx.x == 0) flag_bad_index(a.error);
+    const bool fine = !__syncthreads_or(descends);
     int before = sum - mine;
     for (int w = 0; w < warp; ++w) before += warp_sums[w];
     for (int i = i0; i < i1; ++i) {

@@ -1,0 +1,50 @@
+"""The packed and int8-cache ops at the edges of what their documentation allows: starts in no order, long sequences,
+strides, values of very different sizes."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+from test_gpu_kv_q8 import Cache, assert_within, attend
+from test_gpu_packed import TYPES, Packed, as_type, code, from_type, status
+
+pytestmark = pytest.mark.gpu
+
+# Descending somewhere, though all sequences together have no more rows than the buffer's 100.
+DESCENDING = [[0, 40, 10, 60], [0, 60, 59, 60], [5, 0, 50, 60], [0, 30, 60, 20]]
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("starts", DESCENDING)
+def test_packed_descending_starts_with_rows_to_spare_run_nothing(lz, device, suite, starts, qt, kt):
+    c = Packed(lz, device, suite, 64, 4, 2, [40, 20, 20], [40, 20, 20], qt, kt, tail=20)
+    b = c.buffers()
+    status(lz, device)
+    b[4].Write(np.array(starts, np.int32))
+    c.call(b)
+    assert status(lz, device) == 2
+    assert np.all(c.read(b) == 7.0)
+    b[4].Write(c.q_starts)  # and the next call is right
+    c.call(b)
+    c.check(c.read(b))
+    assert status(lz, device) == 0
+    for x in b:
+        x.Dispose()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("starts", DESCENDING)
+def test_q8_descending_starts_with_rows_to_spare_run_nothing(lz, device, suite, starts, dt):
+    rng = np.random.default_rng(30)
+    c = Cache(lz, device, suite, 3, 128, 2, 64, 32, rng, scale=0.01)
+    st, le = c.int_buffer(starts), c.int_buffer([128, 100, 60])
+    x = as_type(np.full(100 * 256, 3.0), dt)[0]
+    status(lz, device)
+    with lz.SharedBuffer.from_array(device, x, code(lz, dt)) as qb, lz.SharedBuffer.from_array(device, x, code(lz, dt)) as ob:
+        suite.Attention.ExecuteQ8(device, qb, *c.buffers, ob, st, le, 64, 4, 2, 32, 128, 3, 100)
+        assert status(lz, device) == 2
+        assert np.all(from_type(ob.ToArray(), dt) == 3.0)
+    assert_within(*attend(lz, device, suite, c, 4, [40, 20, 30], [128, 100, 60], dt))
+    assert status(lz, device) == 0
+    for b in (st, le):
+        b.Dispose()
+    c.dispose()
