@@ -337,10 +337,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
                                      static_cast<long long>(x.s.q0 + x.tok + min(row0 + r, x.rows - 1)) * a.q_stride +
                                      x.head * HD + lane * (HD / 32);
                     if constexpr (HD == 128) {
-                        const float4 w = __ldg(reinterpret_cast<const float4*>(q));
+                        const float4 w = *reinterpret_cast<const float4*>(q);
                         y[r][0] = w.x; y[r][1] = w.y; y[r][2] = w.z; y[r][3] = w.w;
                     } else {
-                        const float2 w = __ldg(reinterpret_cast<const float2*>(q));
+                        const float2 w = *reinterpret_cast<const float2*>(q);
                         y[r][0] = w.x; y[r][1] = w.y;
                     }
                 }

@@ -72,10 +72,10 @@ struct Walk {
     int slots;  // per tile
 
     __device__ __forceinline__ void sequence(int i, int& row0, int& n, int& len) const {
-        const int s = a.starts ? __ldg(a.starts + i) : i, e = a.starts ? __ldg(a.starts + i + 1) : i + 1;
+        const int s = a.starts ? a.starts[i] : i, e = a.starts ? a.starts[i + 1] : i + 1;
         row0 = clamp_start(s, a.tokens);
         n = max(0, clamp_start(e, a.tokens) - row0);
-        len = max(0, min(__ldg(a.lengths + i), a.max_seq));
+        len = max(0, min(a.lengths[i], a.max_seq));
     }
     __device__ __forceinline__ int column_groups(int n) const { return (n * (a.nh / a.nkv) + 8 * NT - 1) / (8 * NT); }
     __device__ __forceinline__ int tiles_of(int len) const { return max(1, (len + slots - 1) / slots); }
@@ -201,9 +201,9 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
         for (int i = i0; i < i1; ++i) {
             int row0, n, len;
             walk.sequence(i, row0, n, len);
-            descends |= a.starts && __ldg(a.starts + i) > __ldg(a.starts + i + 1);
-            if (blockIdx.x == 0 && (descends || __ldg(a.lengths + i) != len ||
-                                    (a.starts && (__ldg(a.starts + i) < 0 || __ldg(a.starts + i + 1) > a.tokens))))
+            descends |= a.starts && a.starts[i] > a.starts[i + 1];
+            if (blockIdx.x == 0 && (descends || a.lengths[i] != len ||
+                                    (a.starts && (a.starts[i] < 0 || a.starts[i + 1] > a.tokens))))
                 flag_bad_index(a.error);
             units += walk.units(n, len);
             items += walk.column_groups(n);
@@ -311,8 +311,8 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             const int slot = fj * SLOTS + h * 32;
             const long long at = static_cast<long long>(slot >> block_log) * a.nkv;
             const bool holds = slot < fi.len;  // a block behind the sequence has no scale to speak of
-            ks[h] = holds ? __ldg(fks + at) : 0.f;
-            vs[h] = holds ? __ldg(fvs + at) : 0.f;
+            ks[h] = holds ? fks[at] : 0.f;
+            vs[h] = holds ? fvs[at] : 0.f;
         }
         ++issued;
         fj += team_warps;

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
 #pragma unroll
                 for (int i = 0; i < WORDS; i += 4) {
                     uint4 u = make_uint4(0, 0, 0, 0);
-                    if (row0 + g * step < n) u = ld_stream_v4(from + i * 4 / static_cast<int>(sizeof(T)));
+                    if (row0 + g * step < n) u = ld_once_v4(from + i * 4 / static_cast<int>(sizeof(T)));
                     w[g][i] = u.x;
                     w[g][i + 1] = u.y;
                     w[g][i + 2] = u.z;
@@ -210,18 +210,18 @@ __global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p) {
         int before = 0, left = p.count;
         while (left > 0) {
             const int step = (left + 31) / 32, i = before + (lane + 1) * step - 1;
-            const int n = step * __popc(__ballot_sync(0xffffffffu, i < before + left && __ldg(p.starts + i) <= t));
+            const int n = step * __popc(__ballot_sync(0xffffffffu, i < before + left && p.starts[i] <= t));
             before += n;
             left = min(left - n, step - 1);
         }
         seq = before - 1;
         if (seq < 0) return;
-        first = __ldg(p.starts + seq);
-        const int end = __ldg(p.starts + seq + 1);
+        first = p.starts[seq];
+        const int end = p.starts[seq + 1];
         if (lane == 0 && (first < 0 || end > p.tokens)) flag_bad_index(p.error);
         if (t >= end) return;
     }
-    const int pos = __ldg(p.positions + seq);
+    const int pos = p.positions[seq];
     const long long nth = static_cast<long long>(t) - first;  // a start may be any number
     if (pos < 0 || pos + nth >= p.max_seq) {
         if (lane == 0) flag_bad_index(p.error);
@@ -233,30 +233,41 @@ __global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p) {
         const int8_t* src = (which ? p.vc : p.kc) + (static_cast<long long>(seq) * p.max_seq + slot) * kvd;
         const float* scales = (which ? p.vs : p.ks) + (static_cast<long long>(seq) * p.blocks + (slot >> block_log)) * p.nkv;
         T* dst = static_cast<T*>(const_cast<void*>(which ? p.v : p.k)) + t * (which ? p.v_stride : p.k_stride);
-#pragma unroll 4
-        for (int c = lane * VEC; c < kvd; c += 32 * VEC) {
-            const float scale = __ldg(scales + (c >> hd_log));
-            float v[8];
-            uint32_t w[2];
-            if constexpr (VEC == 4) {
-                w[0] = __ldg(reinterpret_cast<const unsigned*>(src + c));
-            } else {
-                const uint2 u = __ldg(reinterpret_cast<const uint2*>(src + c));
-                w[0] = u.x;
-                w[1] = u.y;
+        // Four steps' codes and scales are on their way before the first is written.
+        for (int c0 = lane * VEC; c0 < kvd; c0 += 4 * 32 * VEC) {
+            uint32_t w[4][VEC / 4];
+            float scale[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = c0 + k * 32 * VEC;
+                if (c >= kvd) break;
+                if constexpr (VEC == 4) {
+                    w[k][0] = *reinterpret_cast<const unsigned*>(src + c);
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2*>(src + c);
+                    w[k][0] = u.x;
+                    w[k][1] = u.y;
+                }
+                scale[k] = scales[c >> hd_log];
             }
 #pragma unroll
-            for (int j = 0; j < VEC / 4; ++j) {
-                float2 a, b;
-                dequant_i8x4(w[j], a, b);
-                v[4 * j] = a.x * scale;
-                v[4 * j + 1] = a.y * scale;
-                v[4 * j + 2] = b.x * scale;
-                v[4 * j + 3] = b.y * scale;
+            for (int k = 0; k < 4; ++k) {
+                const int c = c0 + k * 32 * VEC;
+                if (c >= kvd) break;
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < VEC / 4; ++j) {
+                    float2 a, b;
+                    dequant_i8x4(w[k][j], a, b);
+                    v[4 * j] = a.x * scale[k];
+                    v[4 * j + 1] = a.y * scale[k];
+                    v[4 * j + 2] = b.x * scale[k];
+                    v[4 * j + 3] = b.y * scale[k];
+                }
+                // f32 rows go past the L2: 22,167 rows stored and read back took 78.5 us, now 70.7. 16-bit ones would lose 1%.
+                if constexpr (VEC == 4) __stcs(reinterpret_cast<float4*>(dst + c), make_float4(v[0], v[1], v[2], v[3]));
+                else store8(dst + c, v);
             }
-            // f32 rows go past the L2: 22,167 rows stored and read back took 78.5 us, now 70.7. 16-bit ones would lose 1%.
-            if constexpr (VEC == 4) __stcs(reinterpret_cast<float4*>(dst + c), make_float4(v[0], v[1], v[2], v[3]));
-            else store8(dst + c, v);
         }
     }
 }

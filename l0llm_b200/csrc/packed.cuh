@@ -1,4 +1,9 @@
 // Device helpers of the ops over packed sequences (attention_packed.cu, attention_q8.cu, kv_q8.cu).
+//
+// What these ops read - rows, codes, scales, starts, positions, lengths - may come from the kernel just before, and under
+// programmatic dependent launch that kernel still runs while this one starts. So nothing of it is read through the
+// read-only path (ld.global.nc), which asks that memory stays as it is for a kernel's whole life; pdl_wait orders the
+// ordinary loads behind it.
 #pragma once
 
 #include "common.cuh"
@@ -24,6 +29,16 @@ __device__ __forceinline__ int block_find_sequence(const int* starts, int count,
         n += __syncthreads_count(i < count && starts[i] <= t);
     }
     return n - 1;
+}
+
+// 16 bytes that are read once: no L1 allocation.
+__device__ __forceinline__ uint4 ld_once_v4(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p)
+                 : "memory");
+    return r;
 }
 
 // Eight consecutive elements of f32 / f16 / bf16 as f32; p on 16 bytes.

@@ -18,10 +18,10 @@ struct PackedSeq {
 
 __device__ __forceinline__ PackedSeq packed_seq(const PackedAttnParams& a, int i) {
     PackedSeq s;
-    s.q0 = clamp_start(__ldg(a.q_starts + i), a.tokens);
-    s.n = max(0, clamp_start(__ldg(a.q_starts + i + 1), a.tokens) - s.q0);
-    s.k0 = clamp_start(__ldg(a.kv_starts + i), a.kv_tokens);
-    s.m = max(0, clamp_start(__ldg(a.kv_starts + i + 1), a.kv_tokens) - s.k0);
+    s.q0 = clamp_start(a.q_starts[i], a.tokens);
+    s.n = max(0, clamp_start(a.q_starts[i + 1], a.tokens) - s.q0);
+    s.k0 = clamp_start(a.kv_starts[i], a.kv_tokens);
+    s.m = max(0, clamp_start(a.kv_starts[i + 1], a.kv_tokens) - s.k0);
     return s;
 }
 
@@ -35,9 +35,9 @@ __device__ __forceinline__ bool packed_scan(const PackedAttnParams& a, int* pre,
     bool bad = false, descends = false;
     for (int i = i0; i < i1; ++i) {
         mine += units(packed_seq(a, i).n);
-        descends |= __ldg(a.q_starts + i) > __ldg(a.q_starts + i + 1);
-        bad |= descends || __ldg(a.q_starts + i) < 0 || __ldg(a.q_starts + i + 1) > a.tokens || __ldg(a.kv_starts + i) < 0 ||
-               __ldg(a.kv_starts + i + 1) > a.kv_tokens || __ldg(a.kv_starts + i) > __ldg(a.kv_starts + i + 1);
+        descends |= a.q_starts[i] > a.q_starts[i + 1];
+        bad |= descends || a.q_starts[i] < 0 || a.q_starts[i + 1] > a.tokens || a.kv_starts[i] < 0 ||
+               a.kv_starts[i + 1] > a.kv_tokens || a.kv_starts[i] > a.kv_starts[i + 1];
     }
     if (bad && blockIdx.x == 0) flag_bad_index(a.error);
     int sum = mine;
