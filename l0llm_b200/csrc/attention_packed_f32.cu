@@ -320,9 +320,13 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
         uint8_t* stage = stage_s + (warp - 4) * 2048;
         float(*swap)[2][kRows] = reinterpret_cast<float(*)[2][kRows]>(stage_s);
         int made = 0, outs = 0, syncs = 0;
-        auto rows_sync = [&]() {  // all row threads; bounded, as every wait here
+        // All row threads; bounded, as every wait here. Weights go over scores that the row's other thread, in another
+        // warp, has read: the fences order its tensor-memory loads before this thread's stores behind the barrier.
+        auto rows_sync = [&]() {
+            tc_before();
             bar_arrive(rows_bar);
             wait_warp(rows_bar, syncs++ & 1);
+            tc_after();
         };
         // Query terms of a unit: a warp's 16 rows, eight rows' loads in flight, a row spread over the lanes. The scores
         // that read the last unit's terms are done: every row thread has seen its last.
