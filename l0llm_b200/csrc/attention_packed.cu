@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     __shared__ uint32_t bad_s[8][4][4];
     __shared__ int any_bad_s[8];
     __shared__ uint32_t tmem_s;
+    __shared__ int descends_s;
     const PackedAttnParams& a = L.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t bar0 = smem_addr(bars);
@@ -144,6 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
             bar_init(read + 8 * i, 11);  // MMA thread, two guard warps, eight softmax warps
         }
         bar_init_fence();
+        descends_s = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.qmap)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.kmap)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.vmap)) : "memory");
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
     tc_after();
     const uint32_t tmem = tmem_s;
 
-    const bool fine = packed_scan(a, pre, scan_s, [&](int n) { return units_of<PAIR>(a, n); });
+    const bool fine = packed_scan(a, pre, scan_s, &descends_s, [&](int n) { return units_of<PAIR>(a, n); });
     const int total = pre[a.count];
     bool ok = true;  // false once a bounded wait gave up: the role stops
     auto wait = [&](uint32_t bar, uint32_t parity) {

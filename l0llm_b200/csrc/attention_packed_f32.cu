@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
     __shared__ uint32_t bad_s[8][2][4];  // [unit & 7][cut tile]: value rows that are not finite
     __shared__ float factor_s[kRows];
     __shared__ uint32_t tmem_s;
+    __shared__ int descends_s;
     const PackedAttnParams& a = L.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t q_full = smem_addr(bars), kv_full = q_full + 8, kv_empty = kv_full + 8 * R, v_ok = kv_empty + 8 * R;
@@ -140,6 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
             bar_init(read + 8 * i, 11);  // the MMA warp, two guard warps, eight row warps
         }
         bar_init_fence();
+        descends_s = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.kmap)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&L.vmap)) : "memory");
     }
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_f32_kernel(const __grid_co
     // Columns: scores and weight terms 0 and 1 of even and odd tiles, O, third terms of even and odd tiles.
     const uint32_t tmem = tmem_s, o_col = tmem + 2 * kRows, p2_col = tmem + 3 * kRows;
 
-    const bool fine = packed_scan(a, pre, scan_s, [&](int n) { return units_of(a, n); });
+    const bool fine = packed_scan(a, pre, scan_s, &descends_s, [&](int n) { return units_of(a, n); });
     const int total = pre[a.count];
     bool ok = true;  // false once a bounded wait gave up: the role stops
     auto wait = [&](uint32_t bar, uint32_t parity) {
