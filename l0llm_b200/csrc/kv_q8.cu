@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p) {
     }
     const int pos = p.positions[seq];
     const long long nth = static_cast<long long>(t) - first;  // a start may be any number
-    if (pos < 0 || pos + nth >= p.max_seq) {
+    if (pos < 0 || nth < 0 || pos + nth >= p.max_seq) {       // in front of its sequence: starts that descend
         if (lane == 0) flag_bad_index(p.error);
         return;
     }

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import numpy as np
 import pytest
+import seq_oracle as so
 from test_gpu_kv_q8 import Cache, assert_within, attend
 from test_gpu_packed import TYPES, Packed, as_type, code, from_type, status
 
@@ -47,4 +48,28 @@ def test_q8_descending_starts_with_rows_to_spare_run_nothing(lz, device, suite, 
     assert status(lz, device) == 0
     for b in (st, le):
         b.Dispose()
+    c.dispose()
+
+
+@pytest.mark.parametrize("starts", [[50, 60, 10, 20], [64, 70, 3, 3]])
+def test_load_touches_nothing_in_front_of_a_sequence(lz, device, suite, starts):
+    # The search for a row's sequence counts the starts up to it: of starts that descend it may name one that begins
+    # behind the row, whose slots in front of its position lie outside the cache.
+    rng = np.random.default_rng(31)
+    c = Cache(lz, device, suite, 3, 64, 1, 64, 32, rng)
+    st, po = c.int_buffer(starts), c.int_buffer([1, 0, 2])
+    out = [lz.SharedBuffer.from_array(device, np.full(100 * 64, 9, np.float32)) for _ in range(2)]
+    status(lz, device)
+    suite.KvCacheQ8.Load(device, *c.buffers, *out, st, po, 1, 64, 32, 64, 3, 100)
+    assert status(lz, device) == 2
+    for w in range(2):
+        got = out[w].ToArray().reshape(100, 64)
+        want = np.full((100, 64), 9, np.float32)
+        for i in range(3):  # rows of a sequence as its own starts have them, or left as they were
+            for t in range(starts[i], max(starts[i], min(starts[i + 1], 100))):
+                if np.any(got[t] != 9):
+                    want[t] = so.values(c.codes[w][i], c.scales[w][i], 32)[po.ToArray()[i] + t - starts[i], 0].astype(np.float32)
+        np.testing.assert_array_equal(got, want)
+    for x in (st, po, *out):
+        x.Dispose()
     c.dispose()
