@@ -298,7 +298,8 @@ L0B_API l0b_status l0b_attention_execute_packed(l0b_suite* s, l0b_device* d, l0b
  * call is row i of these buffers (l0b_buffer_view names a run of rows). All zero (as allocated) is a valid empty
  * cache. starts: i32 [count + 1], the packed rows of each sequence as in l0b_attention_execute_packed; NULL: one
  * row a sequence (tokens == count). positions / lengths: i32 [count]. All are read on the device, so a recorded
- * command list follows their contents; starts ascend. hd 64 or 128; count <= 4096. Rows of k, v, q, out and of the
+ * command list follows their contents; starts ascend (Store and Load set the error status where they do not, and may
+ * leave out rows of the sequences concerned). hd 64 or 128; count <= 4096. Rows of k, v, q, out and of the
  * cache start on 16 bytes (base and stride).
  *
  * Store: rows of k / v [tokens, nKv * hd] (f32, f16 or bf16, row strides as above) go to slots positions[i],

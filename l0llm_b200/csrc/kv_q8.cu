@@ -28,12 +28,16 @@ __device__ __forceinline__ int code_of_f64(double x, float scale) {
     return static_cast<int>(fmin(127.0, fmax(-127.0, rint(x / static_cast<double>(scale)))));
 }
 
-// Starts that ascend lie inside the buffer if the first and the last do; sequences wholly outside have no row that
-// would show it. The last CTA does this and nothing else: in one that also works it cost 2 us of cold loads.
-__device__ __forceinline__ void check_ends(const KvQ8Params& p) {
-    if (!p.starts || threadIdx.x != 0) return;
-    const int first = p.starts[0], last = p.starts[p.count];
-    if (first != clamp_start(first, p.tokens) || last != clamp_start(last, p.tokens)) flag_bad_index(p.error);
+// Starts outside the rows or descending may leave rows to nobody, who then could not report it. The last CTA looks at
+// all starts and does nothing else: in one that also works the first and the last alone cost 2 us of cold loads.
+__device__ __forceinline__ void check_starts(const KvQ8Params& p) {
+    if (!p.starts) return;
+    bool bad = false;
+    for (int i = threadIdx.x; i <= p.count; i += blockDim.x) {
+        const int start = p.starts[i], next = p.starts[min(i + 1, p.count)];
+        bad |= start != clamp_start(start, p.tokens) || start > next;
+    }
+    if (bad) flag_bad_index(p.error);
 }
 
 template <typename T>
@@ -86,7 +90,7 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
     const int row0 = tid / (HD / 8), col = tid % (HD / 8) * 8, step = blockDim.x / (HD / 8);
     pdl_wait();
     pdl_launch_dependents();
-    if (blockIdx.x == gridDim.x - 1) return check_ends(p);
+    if (blockIdx.x == gridDim.x - 1) return check_starts(p);
 
     const int t0 = range * rows_per_cta, t1 = min(p.tokens, t0 + rows_per_cta);
     int seq = p.starts ? block_find_sequence(p.starts, p.count, t0) : t0;
@@ -201,7 +205,7 @@ __global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p) {
     constexpr int VEC = 16 / sizeof(T);  // codes of a thread's step: 16 bytes out
     pdl_wait();
     pdl_launch_dependents();
-    if (blockIdx.x == gridDim.x - 1) return check_ends(p);
+    if (blockIdx.x == gridDim.x - 1) return check_starts(p);
     const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int kvd = p.nkv * p.hd, hd_log = p.hd == 128 ? 7 : 6, block_log = 31 - __clz(p.block);
     if (t >= p.tokens) return;

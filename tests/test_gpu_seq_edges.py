@@ -73,3 +73,40 @@ def test_load_touches_nothing_in_front_of_a_sequence(lz, device, suite, starts):
     for x in (st, po, *out):
         x.Dispose()
     c.dispose()
+
+
+@pytest.mark.parametrize("starts", [*DESCENDING, [0, 50, 10, 60], [90, 95, 99, 0]])
+def test_store_and_load_report_descending_starts(lz, device, suite, starts):
+    rng = np.random.default_rng(32)
+    c = Cache(lz, device, suite, 3, 128, 1, 64, 32, rng)
+    st, po = c.int_buffer(starts), c.int_buffer([0, 0, 0])
+    x = [lz.SharedBuffer.from_array(device, rng.standard_normal(100 * 64).astype(np.float32)) for _ in range(2)]
+    status(lz, device)
+    suite.KvCacheQ8.Load(device, *c.buffers, *x, st, po, 1, 64, 32, 128, 3, 100)
+    assert status(lz, device) == 2
+    suite.KvCacheQ8.Store(device, *x, *c.buffers, st, po, 1, 64, 32, 128, 3, 100)
+    assert status(lz, device) == 2
+    for b in (st, po, *x):
+        b.Dispose()
+    c.dispose()
+
+
+def test_store_and_load_look_at_every_start(lz, device, suite):
+    # one descending pair among more starts than a CTA has threads
+    count = 1500
+    c = Cache(lz, device, suite, count, 8, 1, 64, 32)
+    x = [lz.SharedBuffer(device, lz.F32, 2 * count * 64) for _ in range(2)]
+    po = c.int_buffer(np.zeros(count))
+    for at in (None, 1, 700, count - 1):
+        starts = np.arange(count + 1)
+        if at is not None:
+            starts[at] += 2
+        st = c.int_buffer(starts)
+        status(lz, device)
+        for op, args in (("Store", (*x, *c.buffers)), ("Load", (*c.buffers, *x))):
+            getattr(suite.KvCacheQ8, op)(device, *args, st, po, 1, 64, 32, 8, count, 2 * count)
+            assert status(lz, device) == (0 if at is None else 2)
+        st.Dispose()
+    for b in (po, *x):
+        b.Dispose()
+    c.dispose()
