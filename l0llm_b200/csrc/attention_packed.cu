@@ -21,6 +21,11 @@
 //
 // Probabilities are rounded once to the operands' type (its MMA takes no other), their sum is taken before that.
 //
+// The MMA truncates its sums, always towards zero: a step of 16 keys costs up to 2^-23 of the sum so far, and 131,072 keys
+// in one sum came out 8.5e-4 low on average, 1,048,576 keys 6.8e-3. So O is summed in tensor memory over 16,384 keys at
+// most (1024 steps, 1.2e-4 at most, 1e-4 measured) and then added to a carry in f32, in global memory, since tensor memory
+// is full and the registers are taken: 128 KB a CTA, written by the row's own thread and read back by it.
+//
 // The tensor cores and the exponentials have as much to do: 2 x 128 x 128 exponentials and four 128 x 128 x HD products
 // take about 2048 cycles each at HD 128. A pair of tiles takes 3250: the MMA warp's waits and commits stand between the
 // products. 16,384 tokens of 64 / 8 heads in bf16 take 3.5 to 4.1 ms (the power limit's share varies), 1.07 to 1.26
@@ -42,11 +47,13 @@ namespace {
 constexpr int kRing = 4;       // K and V tiles in shared memory
 constexpr int kUnitSlots = 4;  // drawn units in flight
 constexpr int kThreads = 384;
+constexpr int kCarryTiles = 128;  // key tiles that O is summed over in tensor memory
 
 struct PackedLaunch {
     CUtensorMap qmap, kmap, vmap;  // [rows, heads * hd], box {64, 128}
     PackedAttnParams a;
     unsigned* counters;  // [0] units drawn beyond each CTA's first, [1] CTAs done; zero at rest
+    float* carry;        // [CTA][query tile][dim][row] sums of O
 };
 
 // One unit, worked out by the drawing thread and handed on in shared memory.
@@ -289,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
 #pragma unroll
                         for (int i = 4 * h; i < 4 * h + 4; ++i)
                             mma_ts(tmem + 2 * kRows + t * HD, tmem + t * kRows + i * 8, n_major_desc(v + i * 2048), kIdescO,
-                                   j > 0 || i > 0);
+                                   j % kCarryTiles > 0 || i > 0);
                     }
                     ++p_uses[t];
                     if (t == (j < x.nt[1] ? 1 : 0)) tc_commit(kv_empty + 8 * st);
@@ -344,15 +351,34 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         const uint32_t s_at = tmem + t * kRows + lanes, o_at = tmem + 2 * kRows + t * HD + lanes;
         const float c = a.scale * 1.44269504088896341f;
         uint8_t* stage = stage_s + (warp - 4) * 2048;
+        float* carry = L.carry + (static_cast<size_t>(blockIdx.x) * 2 + t) * 128 * kRows + row;
         uint32_t s_uses = 0, o_uses = 0;
         for (int i = 0;; ++i) {
             Unit x;
             if (!next_unit(x)) break;
             const int nt = x.nt[t], limit = x.s.m - x.s.n + x.tok[t] + row;  // the last key this row sees
             float ref = kNegInf, sum = 0.f;  // weights are exp2((s - ref) c)
+            float carry_ref = kNegInf;       // the reference that the carry was last written under
+            auto carry_scale = [&]() { return carry_ref == ref ? 1.f : exp2_fast((carry_ref - ref) * c); };
             for (int j = 0; j < nt; ++j) {
                 if (!wait_warp(s_full + 8 * t, s_uses++ & 1)) break;
                 tc_after();
+                const bool anew = j % kCarryTiles == 0;  // O starts anew with this tile
+                if (anew && j > 0) {
+                    const float f = carry_scale();
+#pragma unroll 1
+                    for (int b = 0; b < HD / 32; ++b) {
+                        uint32_t o[32];
+                        tmem_load32(o_at + 32 * b, o);
+                        tmem_loaded(o);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            float* at = carry + (32 * b + k) * kRows;
+                            *at = __uint_as_float(o[k]) + (j > kCarryTiles ? *at * f : 0.f);
+                        }
+                    }
+                    carry_ref = ref;
+                }
                 uint32_t s[4][32];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) tmem_load32(s_at + 32 * b, s[b]);
@@ -375,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                 const bool move = most > ref && !((most - ref) * c <= 8.f);
                 if (__any_sync(0xffffffffu, move)) {
                     const float by = move ? exp2_fast((ref - most) * c) : 1.f;
-                    if (j > 0) {
+                    if (!anew) {
 #pragma unroll 1
                         for (int b = 0; b < HD / 32; ++b) {
                             uint32_t o[32];
@@ -437,6 +463,12 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                 if (b == HD / 32 - 1 && nt > 0) {
                     tc_before();
                     bar_arrive(o_empty + 8 * t);
+                }
+                if (nt > kCarryTiles) {
+                    const float f = carry_scale();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        o[k] = __float_as_uint(fmaf(carry[(32 * b + k) * kRows], f, __uint_as_float(o[k])));
                 }
                 if (row < x.rows[t]) {
                     // Values that the guard set aside, where this row sees them.
@@ -522,6 +554,7 @@ l0b_status launch_tc(l0b_suite* s, l0b_device* d, const PackedAttnParams& a) {
     L0B_TRY(tensor_map_2d(&L.vmap, type, 2, a.v, kvw, kv_rows, a.v_stride, 64, kRows, CU_TENSOR_MAP_SWIZZLE_128B));
     L.a = a;
     L.counters = s->packed_counters;
+    L.carry = s->packed_carry;
     return d->launch(kernel, dim3(d->sm_count), dim3(kThreads), tiles + 4 * (static_cast<size_t>(a.count) + 1), L);
 }
 

@@ -47,6 +47,7 @@ l0b_suite::~l0b_suite() {
     if (q8_part) cudaFree(q8_part);
     if (q8_counters) cudaFree(q8_counters);
     if (packed_counters) cudaFree(packed_counters);
+    if (packed_carry) cudaFree(packed_carry);
 }
 
 namespace {
@@ -109,6 +110,7 @@ L0B_API l0b_status l0b_suite_create(l0b_device* dev, l0b_suite** out) {
     L0B_CHECK_CUDA(cudaMalloc(&s->q8_part, sizeof(float) * 2 * teams * 16 * (128 + 2)));
     L0B_CHECK_CUDA(cudaMalloc(&s->q8_counters, sizeof(unsigned) * teams));
     L0B_CHECK_CUDA(cudaMalloc(&s->packed_counters, sizeof(unsigned) * 2));
+    L0B_CHECK_CUDA(cudaMalloc(&s->packed_carry, sizeof(float) * 2 * 128 * 128 * dev->sm_count));
     L0B_CHECK_CUDA(cudaMemsetAsync(s->packed_counters, 0, sizeof(unsigned) * 2, dev->stream));
     L0B_CHECK_CUDA(cudaMemsetAsync(s->q8_counters, 0, sizeof(unsigned) * teams, dev->stream));
     L0B_CHECK_CUDA(cudaStreamSynchronize(dev->stream));

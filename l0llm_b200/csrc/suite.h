@@ -40,6 +40,7 @@ struct l0b_suite {
     float* q8_part = nullptr;
     unsigned* q8_counters = nullptr;
     unsigned* packed_counters = nullptr;  // packed attention: units drawn, CTAs done; zero at rest
+    float* packed_carry = nullptr;        // packed attention: sums of O, two tiles of 128 rows of 128 dims a CTA
     std::map<std::pair<int, double>, float*> rope_tables;
     ~l0b_suite();
 };

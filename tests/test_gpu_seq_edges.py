@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import seq_oracle as so
 from test_gpu_kv_q8 import Cache, assert_within, attend
-from test_gpu_packed import TYPES, Packed, as_type, code, from_type, status
+from test_gpu_packed import TYPES, UNIT, UNIT_P, Packed, as_type, code, from_type, status
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,75 @@ def test_store_and_load_look_at_every_start(lz, device, suite):
     for b in (po, *x):
         b.Dispose()
     c.dispose()
+
+
+# ----------------------------------------------------------------------------------------------
+# Long sequences
+# ----------------------------------------------------------------------------------------------
+
+def check_long(c, got, floor_p=2.0 ** -38):
+    """Packed.check, with 1024 truncated sums of 2^-23 relative for 16-bit queries: the steps that the MMA sums O over."""
+    out, spread, dot, mass = c.want()
+    bound = so.attention_bound(out, spread, dot, mass, c.hd, UNIT_P[c.qt], UNIT[c.qt], floor_p)
+    if c.qt != "f32":
+        bound += 1024 * 2.0 ** -23 * (np.abs(out) + spread)
+    err = np.abs(got - out)
+    assert np.all(err <= bound), f"{(err / bound).max():.3g} of the bound, max err {err.max():.3g}"
+    return out
+
+
+# Values of one sign, so that truncated sums add up; keys enough for them to pass half a step of the result's type.
+@pytest.mark.parametrize("qt,kt,m,hd,nh", [("f16", "f16", 300000, 64, 2), ("f16", "f16", 300000, 128, 1),
+                                           ("bf16", "bf16", 1200000, 64, 1), ("f32", "f16", 300000, 128, 1),
+                                           ("f32", "bf16", 300000, 64, 2)])
+def test_sums_over_many_keys_do_not_drift(lz, device, suite, qt, kt, m, hd, nh):
+    def edit(q, k, v):
+        q *= 0.1
+        v[:] = np.abs(v) + 0.5
+
+    c = Packed(lz, device, suite, hd, nh, 1, [2], [m], qt, kt, edit=edit)
+    check_long(c, c.run())
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("hd,nh,nkv,m", [(64, 4, 2, 16384), (128, 3, 3, 16385), (128, 2, 1, 16512), (64, 3, 1, 40000)])
+def test_few_rows_behind_a_long_prefix(lz, device, suite, hd, nh, nkv, m, qt, kt):
+    # on both sides of the 128 tiles of one sum, with a reference that moves late: the last keys are the largest
+    def edit(q, k, v):
+        k *= np.linspace(0.2, 3.0, k.shape[0])[:, None]
+
+    c = Packed(lz, device, suite, hd, nh, nkv, [3, 1], [m, 130], qt, kt, edit=edit)
+    check_long(c, c.run())
+
+
+@pytest.mark.parametrize("qt,kt", [("f16", "f16"), ("bf16", "bf16")])
+def test_a_carry_of_rows_that_saw_nothing_or_no_number(lz, device, suite, qt, kt):
+    # a key that is no number in the first sum shows in every row; scores of minus infinity alone there weigh nothing
+    m, hd = 20000, 64
+    for bad in (np.nan, -np.inf):
+        def edit(q, k, v):
+            q[:, 0] = 1.0
+            k[:16384, 0] = bad
+
+        c = Packed(lz, device, suite, hd, 1, 1, [5], [m], qt, kt, edit=edit)
+        with np.errstate(all="ignore"):
+            got = c.run()
+        if np.isnan(bad):
+            assert not np.isfinite(got).any()
+            continue
+        o, *errs = so.attention(c.qv, c.kv[16384:], c.vv[16384:], np.arange(m - 16384 - 5, m - 16384), 1, 1)
+        assert np.all(np.abs(got - o) <= so.attention_bound(o, *errs, hd, UNIT_P[qt], UNIT[qt], 2.0 ** -32))
+
+
+def test_same_bits_of_a_long_sequence_replayed(lz, device, suite):
+    c = Packed(lz, device, suite, 128, 4, 2, [200, 300], [20000, 33000], "bf16", "bf16")
+    b = c.buffers()
+    c.call(b)
+    first = b[3].ToArray()
+    for _ in range(2):
+        device.BeginRecording()
+        c.call(b)
+        device.EndRecording()
+        np.testing.assert_array_equal(b[3].ToArray(), first)
+    for x in b:
+        x.Dispose()
