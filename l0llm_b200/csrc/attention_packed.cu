@@ -19,7 +19,10 @@
 // guard zeroes value rows behind the sequence, and value rows that hold an infinity or a NaN, which it notes; the
 // rows that do see such a key add its share in the epilogue.
 //
-// Probabilities are rounded once to the operands' type (its MMA takes no other), their sum is taken before that.
+// Probabilities are rounded once to the operands' type (its MMA takes no other), their sum is taken before that. f16
+// weights carry a factor 2^7: with the 2^8 that the reference may lag behind, 2^15 is the largest power of two that f16
+// holds, and half of its smallest step is then 2^-32 of the row's largest weight at most. (Without it 131,071 keys at 2^-26
+// of one other's weight, 2^-9 of the result, were lost.)
 //
 // The MMA truncates its sums, always towards zero: a step of 16 keys costs up to 2^-23 of the sum so far, and 131,072 keys
 // in one sum came out 8.5e-4 low on average, 1,048,576 keys 6.8e-3. So O is summed in tensor memory over 16,384 keys at
@@ -47,6 +50,7 @@ namespace {
 constexpr int kRing = 4;       // K and V tiles in shared memory
 constexpr int kUnitSlots = 4;  // drawn units in flight
 constexpr int kThreads = 384;
+template <bool BF> constexpr float kLiftBits = BF ? 0.f : 7.f;  // of the weights
 constexpr int kCarryTiles = 128;  // key tiles that O is summed over in tensor memory
 
 struct PackedLaunch {
@@ -357,7 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
             Unit x;
             if (!next_unit(x)) break;
             const int nt = x.nt[t], limit = x.s.m - x.s.n + x.tok[t] + row;  // the last key this row sees
-            float ref = kNegInf, sum = 0.f;  // weights are exp2((s - ref) c)
+            float ref = kNegInf, sum = 0.f;  // weights are exp2((s - ref) c + kLiftBits)
+            auto shift_of = [&]() { return ref == kNegInf ? 0.f : fmaf(ref, c, -kLiftBits<BF>); };
             float carry_ref = kNegInf;       // the reference that the carry was last written under
             auto carry_scale = [&]() { return carry_ref == ref ? 1.f : exp2_fast((carry_ref - ref) * c); };
             for (int j = 0; j < nt; ++j) {
@@ -397,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                     for (int b = 0; b < 4; ++b) top[b] = fmaxf(fmaxf(top[b], __uint_as_float(s[b][k])), __uint_as_float(s[b][k + 1]));
                 }
                 const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                // The reference moves when it must: at the first keys seen, or when weights would pass 2^8.
+                // The reference moves when it must: at the first keys seen, or when weights would pass 2^8 of it.
                 const bool move = most > ref && !((most - ref) * c <= 8.f);
                 if (__any_sync(0xffffffffu, move)) {
                     const float by = move ? exp2_fast((ref - most) * c) : 1.f;
@@ -418,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                     }
                 }
                 __syncwarp();
-                const float shift = ref == kNegInf ? 0.f : ref * c;
+                const float shift = shift_of();
                 const float2 c2 = make_float2(c, c), shift2 = make_float2(-shift, -shift);
                 float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                             for (uint32_t bits = bad_s[i & 7][nth & 3][w]; bits; bits &= bits - 1) {
                                 const int key = j * kRows + w * 32 + __ffs(bits) - 1;
                                 if (key > limit) break;
-                                const float f = weight_anew<T, HD>(a, x.s, x.head[t], x.tok[t] + row, key, c, ref == kNegInf ? 0.f : ref * c);
+                                const float f = weight_anew<T, HD>(a, x.s, x.head[t], x.tok[t] + row, key, c, shift_of());
                                 const T* v = static_cast<const T*>(a.v) + static_cast<long long>(x.s.k0 + key) * a.v_stride +
                                              x.head[t] / (a.nh / a.nkv) * HD + 32 * b;
 #pragma unroll

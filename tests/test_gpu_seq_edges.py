@@ -141,6 +141,25 @@ def test_sums_over_many_keys_do_not_drift(lz, device, suite, qt, kt, m, hd, nh):
 
 
 @pytest.mark.parametrize("qt,kt", TYPES)
+@pytest.mark.parametrize("hd,nh", [(64, 2), (128, 1)])
+def test_many_small_weights_beside_a_large_one(lz, device, suite, hd, nh, qt, kt):
+    # One key at about 2^26 times the weight of 131,071 others, its value 0: what is left is the sum of the small ones.
+    # f16 weights keep steps of 2^-24 under a factor of 2^7 at least: half a step is 2^-32 of the largest weight.
+    def edit(q, k, v):
+        q[:, 0::hd] = 16.0
+        q[:, 1:hd] *= 0.5
+        k[:, 0] = 0
+        k[0] = 0
+        k[0, 0] = 26 * np.log(2) * np.sqrt(hd) / 16
+        v[:] = np.abs(v) + 0.5
+        v[0] = 0
+
+    c = Packed(lz, device, suite, hd, nh, 1, [2], [131072], qt, kt, edit=edit)
+    out = check_long(c, c.run(), floor_p=2.0 ** -32 if qt == "f16" else 2.0 ** -38)
+    assert np.all(out > 2.0 ** -11)
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
 @pytest.mark.parametrize("hd,nh,nkv,m", [(64, 4, 2, 16384), (128, 3, 3, 16385), (128, 2, 1, 16512), (64, 3, 1, 40000)])
 def test_few_rows_behind_a_long_prefix(lz, device, suite, hd, nh, nkv, m, qt, kt):
     # on both sides of the 128 tiles of one sum, with a reference that moves late: the last keys are the largest
