@@ -325,9 +325,11 @@ L0B_API l0b_status l0b_kv_cache_q8_load(l0b_suite* s, l0b_device* d, l0b_buffer*
 /* Attention.Execute over the int8 cache for `count` sequences at once: sequence i holds lengths[i] slots, the last
  * of them the positions of its n query rows (one, or a few drafted tokens), and query t attends to slots
  * [0, lengths[i] - n + t] (none: zeros). q [tokens, nH * hd] and out: f32, f16 or bf16, one type; row strides in
- * elements (<= 0: packed rows). Products and sums keep about f32 accuracy against the cache's values. Starts that
- * descend anywhere run nothing and set the error status. One launch for any mix of lengths. Long blocks of queries are
- * better served by Load and l0b_attention_execute_packed. */
+ * elements (<= 0: packed rows). Products and sums keep about f32 accuracy against the cache's values: a query value
+ * enters as an integer of 31 bits of the largest of its row and head (bf16: 23 bits; off by 2^-30, or 2^-22, of that
+ * largest at most), sums are exact or f32, weights two f16 terms (bf16: one, so 2^-11 relative). Starts that descend
+ * anywhere run nothing and set the error status. One launch for any mix of lengths. Long blocks of queries are better
+ * served by Load and l0b_attention_execute_packed. */
 L0B_API l0b_status l0b_attention_execute_q8(l0b_suite* s, l0b_device* d, l0b_buffer* q, l0b_buffer* kc,
                                             l0b_buffer* vc, l0b_buffer* k_scales, l0b_buffer* v_scales,
                                             l0b_buffer* out, l0b_buffer* starts, l0b_buffer* lengths,

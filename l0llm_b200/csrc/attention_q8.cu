@@ -11,8 +11,8 @@
 //
 // The query columns of an item are the rows that share its keys (the heads of a group, times the tokens): the MMA's
 // n = 8 (NT tiles of it). Keys are its m: S^T[16 slots, 8 columns] = K Q^T on the integer MMA, the codes as they lie
-// in the cache and each query column as three base-256 digits of its values, scaled by a power of two to 23 bits of
-// the column's largest: exact sums and no conversion (turning keys to f16 took 160 of 790 instructions a tile).
+// in the cache and each query column as base-256 digits of its values, scaled by a power of two to 31 bits (bf16: 23)
+// of the column's largest: exact sums and no conversion (turning keys to f16 took 160 of 790 instructions a tile).
 // O^T[16 dims, 8] += V^T P^T takes the codes as f16, exactly (byte b ^ 0x80 under the exponent of 1024, minus 1152),
 // and P^T in hi + lo f16 terms made from the scores' own registers by movmatrix; digits there would cost more than
 // they save, since every output would have to be converted for every tile. No product is padded to 16 query rows,
@@ -163,7 +163,13 @@ __device__ __forceinline__ void team_sync(int id, int threads) {
 // weight to f16 (2^-12) is not seen, and 60 instructions a tile fall away.
 template <typename T>
 constexpr bool kWeightPairs = DT<T>::id != L0B_BF16;
-constexpr int kDigits = 3;  // of a query value
+// Digits of a query value. What they drop is relative to the column's LARGEST value (2^-30 of it at most with four, 2^-22
+// with three), so a loud channel costs the others bits: beside one of 1e4 three digits were off by 1e-4 of the largest
+// output, 19 times the bound of f32 sums. Four keep every bit of values down to 2^-7 of the largest, f16's down to 2^-19.
+// Three hold a bf16 value's 8 bits down to 2^-14 of the largest. The fourth costs 6% (41,159 slots of 4 heads 27.9 -> 29.5
+// us in f32, 514,036 of 8 heads 220 -> 237 us in bf16).
+template <typename T>
+constexpr int kDigits = DT<T>::id == L0B_BF16 ? 3 : 4;
 
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __grid_constant__ Q8Launch L) {
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     constexpr int SLOTS = kTileBytes / HD, MT = SLOTS / 16, HALVES = SLOTS / 32;
     constexpr int KS = HD / 32;   // 32-deep steps of K Q^T
     constexpr int DT_ = HD / 16;  // 16-dim tiles of O
-    constexpr int ND = kDigits;
+    constexpr int ND = kDigits<T>, kTopBit = ND == 4 ? 30 : 22, kBias = ND == 4 ? 0x808080 : 0x8080;
     constexpr bool PAIRS = kWeightPairs<T>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -366,11 +372,11 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             if (odd) top = __int_as_float(0x7F800000);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^bits lifts the column's largest value to 2^21 or more and at most 127 2^16: three signed digits.
+            // 2^bits lifts the column's largest value to 2^(kTopBit - 1) or more, and at most a top digit of 127.
             int bits = 0;
             if (top > 0.f && top < __int_as_float(0x7F800000)) {
-                bits = min(22 - ilogbf(top), 126);
-                if (ldexpf(top, bits) > 127.f * 65536.f) --bits;
+                bits = min(kTopBit - ilogbf(top), 126);
+                if (ldexpf(top, bits) > 127.f * (1 << (kTopBit - 6))) --bits;
             }
             float f = ldexpf(a.scale * 1.44269504088896341f, -bits);
             if (top == __int_as_float(0x7F800000)) f = __int_as_float(0x7FC00000);
@@ -381,7 +387,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                 for (int b = 0; b < 2; ++b) {
                     int v[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = (__float2int_rn(x[8 * s + 4 * b + i] * up) + 0x8080) ^ 0x8080;
+                    for (int i = 0; i < 4; ++i) v[i] = (__float2int_rn(x[8 * s + 4 * b + i] * up) + kBias) ^ kBias;
 #pragma unroll
                     for (int k = 0; k < ND; ++k) qd[nt][s][k][b] = byte_of(v, k);
                 }
@@ -454,12 +460,12 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                             }
                         }
                     }
-                    // d0 + 256 d1 stays below 2^30, so one conversion takes both
+                    // d0 + 256 d1 stays below 2^30, d2 + 256 d3 too: a conversion for each two
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            sc[nt][mt][i] = fmaf(static_cast<float>(acc[nt][2][i]), 65536.f,
+                            sc[nt][mt][i] = fmaf(static_cast<float>((ND == 4 ? acc[nt][ND - 1][i] * 256 : 0) + acc[nt][2][i]), 65536.f,
                                                  static_cast<float>(acc[nt][1][i] * 256 + acc[nt][0][i]));
                 }
             }

@@ -5,6 +5,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 import seq_oracle as so
+from test_gpu_kv_q8 import UNIT_P as Q8_UNIT_P
 from test_gpu_kv_q8 import Cache, assert_within, attend
 from test_gpu_packed import TYPES, UNIT, UNIT_P, Packed, as_type, code, from_type, status
 
@@ -201,3 +202,45 @@ def test_same_bits_of_a_long_sequence_replayed(lz, device, suite):
         np.testing.assert_array_equal(b[3].ToArray(), first)
     for x in b:
         x.Dispose()
+
+
+# ----------------------------------------------------------------------------------------------
+# Attention over the int8 cache
+# ----------------------------------------------------------------------------------------------
+
+def attend_rows(lz, device, suite, c, nh, q, n, lengths, dt, stride=0):
+    """ExecuteQ8 of the rows q [sum(n), nh * hd] (strided by `stride` elements where given); (got, want, bound)."""
+    rows, width = q.shape
+    qs, qv = as_type(q, dt)
+    held = qs if not stride else np.pad(qs, ((0, 0), (0, stride - width)))
+    st, le = c.int_buffer(np.concatenate([[0], np.cumsum(n)])), c.int_buffer(lengths)
+    with lz.SharedBuffer.from_array(device, held, code(lz, dt)) as qb, lz.SharedBuffer(device, code(lz, dt), rows * width) as ob:
+        suite.Attention.ExecuteQ8(device, qb, *c.buffers, ob, st, le, c.hd, nh, c.nkv, c.block, c.max_seq, c.count, rows, stride)
+        got = from_type(ob.ToArray(), dt).reshape(rows, nh, c.hd)
+    for x in (st, le):
+        x.Dispose()
+    want, bound, a = np.zeros(got.shape), np.zeros(got.shape), 0
+    for i, (m, length) in enumerate(zip(n, lengths)):
+        k, v = (so.values(c.codes[w][i][:length], c.scales[w][i], c.block).reshape(length, -1) for w in range(2))
+        o, *errs = so.attention(qv[a:a + m], k, v, np.arange(length - m, length), nh, c.nkv)
+        want[a:a + m], bound[a:a + m] = o, so.attention_bound(o, *errs, c.hd, Q8_UNIT_P[dt], UNIT[dt])
+        a += m
+    return got, want, bound
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,nh,n", [(128, 4, [1, 1]), (64, 14, [1, 3])])
+@pytest.mark.parametrize("loud,key", [(1e2, 0), (1e3, 0), (1e4, 0), (1e3, 1)])
+def test_q8_queries_with_a_loud_channel(lz, device, suite, loud, key, hd, nh, n, dt):
+    # A query channel far above the others where the keys' codes are 0 or tiny: the others make the score, and keep
+    # the accuracy of a sum in f32 that never met the loud one. Queries enter as integers of 31 bits of the largest (bf16:
+    # 23): at 1e4 the others of size 1 are off by 2^-17 each at most, on terms of random sign; the bound has (hd / 8 + 4)
+    # 2^-23 of the sum of all magnitudes (bf16: 2^-9, less than half a step of its values, and its weights' 2^-11).
+    rng = np.random.default_rng(40)
+    c = Cache(lz, device, suite, 2, 300, 2, hd, 64, rng, scale=0.01)
+    c.codes[0][..., 5] = key * rng.integers(-1, 2, c.codes[0][..., 5].shape)
+    c.buffers[0].Write(c.codes[0])
+    q = rng.standard_normal((sum(n), nh * hd))
+    q[:, 5::hd] = loud
+    assert_within(*attend_rows(lz, device, suite, c, nh, q, n, [300, 170], dt))
+    c.dispose()
