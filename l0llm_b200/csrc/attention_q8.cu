@@ -683,7 +683,8 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
             if (whole) {
                 const int tok = (c0 + c) / G, head = c0 + c - tok * G;
                 T* out = static_cast<T*>(a.out) + (it.row0 + tok) * a.out_stride + (kvh * G + head) * HD + x * 4;
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                // A row without slots gives zeros; one whose every score is -inf has no weights, and 0 / 0 says so.
+                const float inv = it.len - it.n + tok < 0 ? 0.f : 1.f / sum;
                 if constexpr (sizeof(T) == 4) {
                     *reinterpret_cast<float4*>(out) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
                 } else {
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
                     }
                     const int tok = (c0 + c) / G, head = c0 + c - tok * G;
                     T* out = static_cast<T*>(a.out) + (it.row0 + tok) * a.out_stride + (kvh * G + head) * HD + x * 4;
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    const float inv = it.len - it.n + tok < 0 ? 0.f : 1.f / sum;
                     if constexpr (sizeof(T) == 4) {
                         *reinterpret_cast<float4*>(out) = make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
                     } else {

@@ -244,3 +244,24 @@ def test_q8_queries_with_a_loud_channel(lz, device, suite, loud, key, hd, nh, n,
     q[:, 5::hd] = loud
     assert_within(*attend_rows(lz, device, suite, c, nh, q, n, [300, 170], dt))
     c.dispose()
+
+
+@pytest.mark.parametrize("length", [20, 3000])  # one part, and parts that are joined
+def test_q8_a_row_whose_scores_are_all_minus_infinity(lz, device, suite, length):
+    # it sees slots, so it is not a row of zeros: its scores pass the range of f32
+    rng = np.random.default_rng(41)
+    c = Cache(lz, device, suite, 2, 3000, 2, 64, 32, rng, scale=0.01)
+    c.codes[0][:] = 100
+    c.buffers[0].Write(c.codes[0])
+    st, le = c.int_buffer([0, 2, 3]), c.int_buffer([length, 0])
+    q = rng.standard_normal((3, 4, 64)).astype(np.float32)
+    q[0, 1] = -3e38
+    with lz.SharedBuffer.from_array(device, q) as qb, lz.SharedBuffer(device, lz.F32, q.size) as ob:
+        suite.Attention.ExecuteQ8(device, qb, *c.buffers, ob, st, le, 64, 4, 2, 32, 3000, 2, 3)
+        got = ob.ToArray().reshape(q.shape)
+    assert np.all(np.isnan(got[0, 1]))
+    got[0, 1] = 1
+    assert np.all(np.isfinite(got)) and not got[2].any()
+    for x in (st, le):
+        x.Dispose()
+    c.dispose()
