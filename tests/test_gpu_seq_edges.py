@@ -265,3 +265,145 @@ def test_q8_a_row_whose_scores_are_all_minus_infinity(lz, device, suite, length)
     for x in (st, le):
         x.Dispose()
     c.dispose()
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("count,length,nh,nkv,hd", [(1, 20000, 8, 1, 128), (3, 6000, 14, 2, 64), (40, 700, 8, 8, 128)])
+def test_q8_long_contexts_of_16_bit_queries(lz, device, suite, count, length, nh, nkv, hd, dt):
+    rng = np.random.default_rng(length)
+    c = Cache(lz, device, suite, count, length, nkv, hd, 64, rng, scale=0.01)
+    lengths = [max(1, length - 997 * i % length) for i in range(count)]
+    assert_within(*attend(lz, device, suite, c, nh, [1] * count, lengths, dt))
+    c.dispose()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,nh,nkv,block", [(128, 28, 4, 64), (64, 9, 3, 128)])
+def test_q8_several_strided_rows_a_sequence(lz, device, suite, hd, nh, nkv, block, dt):
+    rng = np.random.default_rng(42)
+    c = Cache(lz, device, suite, 4, 260, nkv, hd, block, rng, scale=0.01)
+    n, lengths = [5, 0, 17, 9], [5, 77, 260, 3]  # the last has rows that see nothing
+    q = rng.standard_normal((sum(n), nh * hd))
+    got, want, bound = attend_rows(lz, device, suite, c, nh, q, n, lengths, dt, stride=nh * hd + 24)
+    assert_within(got, want, bound)
+    assert not got[-9:-3].any()
+    c.dispose()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("which", [0, 1])  # scales of keys, of values
+def test_q8_a_scale_that_is_not_finite_shows_in_its_heads_alone(lz, device, suite, which, bad):
+    rng = np.random.default_rng(43)
+    c = Cache(lz, device, suite, 2, 300, 2, 64, 32, rng, scale=0.01)
+    before, *_ = attend(lz, device, suite, c, 6, [1, 2], [300, 200], "f32")
+    c.scales[which][1, 3, 1] = bad  # a block that both rows of the second sequence see, of the second KV head
+    c.buffers[2 + which].Write(c.scales[which])
+    with np.errstate(all="ignore"):
+        after, *_ = attend(lz, device, suite, c, 6, [1, 2], [300, 200], "f32")
+    assert not np.isfinite(after[1:, 3:]).any()
+    after[1:, 3:] = before[1:, 3:]
+    np.testing.assert_array_equal(after, before)
+    c.dispose()
+
+
+def test_q8_accuracy_behind_offsets_past_32_bits(lz, device, suite):
+    # The second sequence's codes start behind 2^31 bytes; 2.2 million slots score 0 with a value of 0, 150 are stored.
+    max_seq, nkv, hd, block, n = 2_200_000, 8, 128, 128, 150
+    assert max_seq * nkv * hd > 2 ** 31
+    blocks, pos = -(-max_seq // block), max_seq - n
+    rng = np.random.default_rng(44)
+    bufs = [lz.SharedBuffer(device, lz.I8, 2 * max_seq * nkv * hd) for _ in range(2)]
+    bufs += [lz.SharedBuffer(device, lz.F32, 2 * blocks * nkv) for _ in range(2)]
+    k, v = (rng.standard_normal((n, nkv * hd)).astype(np.float32) for _ in range(2))
+    ints = [lz.SharedBuffer.from_array(device, np.array(x, np.int32)) for x in ([0, 0, n], [0, pos], [0, max_seq], [0, 0, 1])]
+    kb, vb, ko, vo = (lz.SharedBuffer.from_array(device, x) for x in (k, v, k * 0, v * 0))
+    suite.KvCacheQ8.Store(device, kb, vb, *bufs, *ints[:2], nkv, hd, block, max_seq, 2, n)
+    suite.KvCacheQ8.Load(device, *bufs, ko, vo, *ints[:2], nkv, hd, block, max_seq, 2, n)
+    q = (rng.standard_normal((1, nkv * hd)) * 8).astype(np.float32)
+    with lz.SharedBuffer.from_array(device, q) as qb, lz.SharedBuffer(device, lz.F32, nkv * hd) as ob:
+        suite.Attention.ExecuteQ8(device, qb, *bufs, ob, ints[3], ints[2], hd, nkv, nkv, block, max_seq, 2, 1)
+        got = ob.ToArray().reshape(nkv, hd)
+    kk, vv = (b.ToArray().reshape(n, nkv, hd).astype(np.float64) for b in (ko, vo))
+    s = np.einsum("jhd,hd->hj", kk, q.reshape(nkv, hd).astype(np.float64)) / np.sqrt(hd)
+    w = np.exp(s)
+    p = w / (w.sum(1, keepdims=True) + (max_seq - n))
+    out, spread = np.einsum("hj,jhd->hd", p, vv), np.sqrt(np.einsum("hj,jhd->hd", p * p, vv * vv))
+    dot = np.abs(kk * q.reshape(nkv, hd)).sum(2).max(0) / np.sqrt(hd)
+    bound = so.attention_bound(out, spread, dot, np.abs(vv).sum(0), hd, Q8_UNIT_P["f32"], UNIT["f32"])
+    # and the result is one of weights that were summed in f32 over a run: 2.2 million / (148 SMs x 12 warps / 8 heads)
+    # slots a warp are 310 tiles, of which a rounding of 2^-24 each can only shrink or grow all outputs alike
+    assert_within(got, out, bound + 310 * 2.0 ** -24 * np.abs(out))
+    for x in (*ints, kb, vb, ko, vo, *bufs):
+        x.Dispose()
+
+
+# ----------------------------------------------------------------------------------------------
+# Strides, and rows past 2^31 elements
+# ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,nkv,block", [(64, 2, 32), (128, 3, 128)])
+def test_store_and_load_of_strided_rows(lz, device, suite, hd, nkv, block, dt):
+    rng = np.random.default_rng(45)
+    c = Cache(lz, device, suite, 3, 200, nkv, hd, block)
+    width, strides = nkv * hd, (nkv * hd + 8, nkv * hd + 40)
+    n, pos = [130, 0, 37], [3, 0, 100]
+    rows = sum(n)
+    stored, values = zip(*(as_type(rng.standard_normal((rows, width)), dt) for _ in range(2)))
+    st, po = c.int_buffer(np.concatenate([[0], np.cumsum(n)])), c.int_buffer(pos)
+    x = [lz.SharedBuffer.from_array(device, np.pad(y, ((0, 0), (0, s - width)), constant_values=7), code(lz, dt))
+         for y, s in zip(stored, strides)]
+    out = [lz.SharedBuffer(device, code(lz, dt), rows * s) for s in strides]
+    suite.KvCacheQ8.Store(device, *x, *c.buffers, st, po, nkv, hd, block, 200, 3, rows, *strides)
+    c.store_model(*values, n, pos)
+    c.check()
+    suite.KvCacheQ8.Load(device, *c.buffers, *out, st, po, nkv, hd, block, 200, 3, rows, *strides)
+    for w in range(2):
+        got = from_type(out[w].ToArray(), dt).reshape(rows, strides[w])
+        want = np.concatenate([so.values(c.codes[w][i], c.scales[w][i], block)[p:p + m] for i, (m, p) in enumerate(zip(n, pos))])
+        want = from_type(as_type(want.reshape(rows, width).astype(np.float32), dt)[0], dt)
+        np.testing.assert_array_equal(got[:, :width], want)
+        assert not got[:, width:].any()
+    assert status(lz, device) == 0
+    for b in (st, po, *x, *out):
+        b.Dispose()
+    c.dispose()
+
+
+@pytest.mark.parametrize("qt,kt", TYPES)
+def test_packed_strides_of_their_own(lz, device, suite, qt, kt):
+    hd, nh, nkv, n, m = 64, 6, 2, [90, 41, 3], [90, 141, 700]
+    c = Packed(lz, device, suite, hd, nh, nkv, n, m, qt, kt)
+    strides = [nh * hd + 8, nkv * hd + 16, nkv * hd + 40, nh * hd + 24]
+    wide = [np.pad(x, ((0, 0), (0, s - x.shape[1]))) for x, s in zip((c.q, c.k, c.v), strides)]
+    b = [lz.SharedBuffer.from_array(device, x, code(lz, t)) for x, t in zip(wide, (qt, kt, kt))]
+    b += [lz.SharedBuffer(device, code(lz, qt), c.tokens * strides[3])]
+    b += [lz.SharedBuffer.from_array(device, x) for x in (c.q_starts, c.kv_starts)]
+    suite.Attention.ExecutePacked(device, *b, hd, nh, nkv, 3, c.tokens, c.kv_tokens, *strides)
+    got = from_type(b[3].ToArray(), qt).reshape(c.tokens, strides[3])
+    assert not got[:, nh * hd:].any()
+    np.testing.assert_array_equal(got[:, :nh * hd].reshape(c.tokens, nh, hd), c.run())
+    for x in b:
+        x.Dispose()
+
+
+@pytest.mark.parametrize("qt,kt", [("f16", "f16"), ("f32", "bf16")])
+def test_packed_rows_past_2_to_the_31_elements(lz, device, suite, qt, kt):
+    c = Packed(lz, device, suite, 64, 2, 1, [100, 40], [100, 40], qt, kt)
+    stride, rows = 1 << 24, 140
+    assert (rows - 1) * stride > 2 ** 31
+    b = []
+    for x, t in ((c.q, qt), (c.k, kt), (c.v, kt), (None, qt)):
+        b.append(lz.SharedBuffer(device, code(lz, t), (rows - 1) * stride + 128))
+        for r in range(rows if x is not None else 0):
+            with b[-1].View(r * stride, x.shape[1]) as row:
+                row.Write(x[r])
+    b += [lz.SharedBuffer.from_array(device, x) for x in (c.q_starts, c.kv_starts)]
+    suite.Attention.ExecutePacked(device, *b, 64, 2, 1, 2, rows, rows, *[stride] * 4)
+    got = []
+    for r in range(rows):
+        with b[3].View(r * stride, 128) as row:
+            got.append(from_type(row.ToArray(), qt))
+    np.testing.assert_array_equal(np.stack(got).reshape(rows, 2, 64), c.run())
+    for x in b:
+        x.Dispose()
