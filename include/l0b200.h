@@ -280,7 +280,7 @@ L0B_API l0b_status l0b_attention_execute_prefill(l0b_suite* s, l0b_device* d, l0
  * in elements (<= 0: packed rows), so q, k and v may be column views of one stacked projection. Rows of q, k, v and
  * out start on 16 bytes (base and stride). hd 64 or 128; count <= 4096. out must not overlap the inputs.
  * f32 queries keep about f32 accuracy (queries and probabilities enter the MMA as sums of 16-bit terms); 16-bit
- * queries meet probabilities rounded to their own type, summed in f32 (truncating, by 2^-13 of the sum at most, however
+ * queries meet probabilities rounded to their own type, summed in f32 (truncating, by 3.1e-4 of the sum at most, however
  * many the keys). A masked key's or value's contents never
  * reach a row, whatever they are; a row that does see a key or value that is not finite need not be finite.
  * Query starts that descend anywhere run nothing and set the error status; a sequence whose key starts descend has no

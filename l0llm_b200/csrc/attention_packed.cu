@@ -24,10 +24,12 @@
 // holds, and half of its smallest step is then 2^-32 of the row's largest weight at most. (Without it 131,071 keys at 2^-26
 // of one other's weight, 2^-9 of the result, were lost.)
 //
-// The MMA truncates its sums, always towards zero: a step of 16 keys costs up to 2^-23 of the sum so far, and 131,072 keys
-// in one sum came out 8.5e-4 low on average, 1,048,576 keys 6.8e-3. So O is summed in tensor memory over 16,384 keys at
-// most (1024 steps, 1.2e-4 at most, 1e-4 measured) and then added to a carry in f32, in global memory, since tensor memory
-// is full and the registers are taken: 128 KB a CTA, written by the row's own thread and read back by it.
+// The MMA truncates, always towards zero: seen on values chosen for it, a step of 16 keys cuts each product at about 2^-25
+// of the sum and the sum at 2^-23, so it costs 5 * 2^-23 of the sum at most. 131,072 keys alike in one sum came out 8.5e-4
+// low, 1,048,576 keys 6.8e-3. So O is summed in tensor memory over 8192 keys at most (512 steps: 3.1e-4 at most, less than
+// half a step of f16; 5e-5 for keys alike) and then added to a carry in f32, in global memory, since tensor memory is full
+// and the registers are taken: 128 KB a CTA, written by the row's own thread and read back by it. One carry a row costs 16,384
+// tokens 2% (4.10 -> 4.18 ms); over 16,384 keys at a time they would need none, but could lose more than f16's half step.
 //
 // The tensor cores and the exponentials have as much to do: 2 x 128 x 128 exponentials and four 128 x 128 x HD products
 // take about 2048 cycles each at HD 128. A pair of tiles takes 3250: the MMA warp's waits and commits stand between the
@@ -51,13 +53,13 @@ constexpr int kRing = 4;       // K and V tiles in shared memory
 constexpr int kUnitSlots = 4;  // drawn units in flight
 constexpr int kThreads = 384;
 template <bool BF> constexpr float kLiftBits = BF ? 0.f : 7.f;  // of the weights
-constexpr int kCarryTiles = 128;  // key tiles that O is summed over in tensor memory
+constexpr int kCarryTiles = 64;  // key tiles that O is summed over in tensor memory
 
 struct PackedLaunch {
     CUtensorMap qmap, kmap, vmap;  // [rows, heads * hd], box {64, 128}
     PackedAttnParams a;
     unsigned* counters;  // [0] units drawn beyond each CTA's first, [1] CTAs done; zero at rest
-    float* carry;        // [CTA][query tile][dim][row] sums of O
+    float* carry;        // [CTA][query tile][dim / 4][row][4] sums of O
 };
 
 // One unit, worked out by the drawing thread and handed on in shared memory.
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
         const uint32_t s_at = tmem + t * kRows + lanes, o_at = tmem + 2 * kRows + t * HD + lanes;
         const float c = a.scale * 1.44269504088896341f;
         uint8_t* stage = stage_s + (warp - 4) * 2048;
-        float* carry = L.carry + (static_cast<size_t>(blockIdx.x) * 2 + t) * 128 * kRows + row;
+        float* carry = L.carry + (static_cast<size_t>(blockIdx.x) * 2 + t) * 128 * kRows + row * 4;
         uint32_t s_uses = 0, o_uses = 0;
         for (int i = 0;; ++i) {
             Unit x;
@@ -377,9 +379,15 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                         tmem_load32(o_at + 32 * b, o);
                         tmem_loaded(o);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            float* at = carry + (32 * b + k) * kRows;
-                            *at = __uint_as_float(o[k]) + (j > kCarryTiles ? *at * f : 0.f);
+                        for (int k = 0; k < 32; k += 4) {
+                            float4* at = reinterpret_cast<float4*>(carry + (32 * b + k) * kRows);
+                            float4 w = make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
+                                                   __uint_as_float(o[k + 3]));
+                            if (j > kCarryTiles) {
+                                const float4 was = *at;
+                                w = make_float4(fmaf(was.x, f, w.x), fmaf(was.y, f, w.y), fmaf(was.z, f, w.z), fmaf(was.w, f, w.w));
+                            }
+                            *at = w;
                         }
                     }
                     carry_ref = ref;
@@ -472,8 +480,13 @@ __global__ void __launch_bounds__(kThreads, 1) packed_tc_kernel(const __grid_con
                 if (nt > kCarryTiles) {
                     const float f = carry_scale();
 #pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        o[k] = __float_as_uint(fmaf(carry[(32 * b + k) * kRows], f, __uint_as_float(o[k])));
+                    for (int k = 0; k < 32; k += 4) {
+                        const float4 was = *reinterpret_cast<const float4*>(carry + (32 * b + k) * kRows);
+                        o[k] = __float_as_uint(fmaf(was.x, f, __uint_as_float(o[k])));
+                        o[k + 1] = __float_as_uint(fmaf(was.y, f, __uint_as_float(o[k + 1])));
+                        o[k + 2] = __float_as_uint(fmaf(was.z, f, __uint_as_float(o[k + 2])));
+                        o[k + 3] = __float_as_uint(fmaf(was.w, f, __uint_as_float(o[k + 3])));
+                    }
                 }
                 if (row < x.rows[t]) {
                     // Values that the guard set aside, where this row sees them.

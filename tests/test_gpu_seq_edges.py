@@ -118,7 +118,8 @@ def test_store_and_load_look_at_every_start(lz, device, suite):
 # ----------------------------------------------------------------------------------------------
 
 def check_long(c, got, floor_p=2.0 ** -38):
-    """Packed.check, with 1024 truncated sums of 2^-23 relative for 16-bit queries: the steps that the MMA sums O over."""
+    """Packed.check, with what the MMA cuts off O for 16-bit queries: 5 * 2^-23 of the sum at most for each of the 512
+    steps that it is summed over, and no more than 2 * 2^-23 of them on average for keys alike."""
     out, spread, dot, mass = c.want()
     bound = so.attention_bound(out, spread, dot, mass, c.hd, UNIT_P[c.qt], UNIT[c.qt], floor_p)
     if c.qt != "f32":
@@ -158,6 +159,28 @@ def test_many_small_weights_beside_a_large_one(lz, device, suite, hd, nh, qt, kt
     c = Packed(lz, device, suite, hd, nh, 1, [2], [131072], qt, kt, edit=edit)
     out = check_long(c, c.run(), floor_p=2.0 ** -32 if qt == "f16" else 2.0 ** -38)
     assert np.all(out > 2.0 ** -11)
+
+
+@pytest.mark.parametrize("qt,kt,m", [("f16", "f16", 262144), ("bf16", "bf16", 1048576), ("f32", "f16", 262144)])
+def test_many_small_keys_behind_a_large_one_in_the_sum(lz, device, suite, qt, kt, m):
+    # The first key's share of O is about 1, each other's below what a truncated sum next to it holds: lost in the first
+    # 512 steps alone (5 * 2^-23 of the sum for each of them at most), not in all.
+    def edit(q, k, v):
+        q[:, 0] = 16.0
+        q[:, 1:] *= 0.5
+        k[:, 0] = 0
+        k[0] = 0
+        k[0, 0] = 25.5 * np.log(2) * 8 / 16
+        v[:] = np.abs(v) + 0.5
+        v[0] = 1
+
+    c = Packed(lz, device, suite, 64, 1, 1, [1], [m], qt, kt, edit=edit)
+    out, spread, dot, mass = c.want()
+    bound = so.attention_bound(out, spread, dot, mass, 64, UNIT_P[qt], UNIT[qt], 2.0 ** -32 if qt == "f16" else 2.0 ** -38)
+    if qt != "f32":
+        bound += 512 * 5 * 2.0 ** -23 * out
+    err = np.abs(c.run() - out)
+    assert np.all(err <= bound), f"{(err / bound).max():.3g} of the bound, max err {err.max():.3g}"
 
 
 @pytest.mark.parametrize("qt,kt", TYPES)
