@@ -3,8 +3,10 @@
 //
 // A unit of work is two tiles of 128 query rows of one sequence that read the same keys: two query heads of one KV
 // head over the same rows where the group is even (PAIR), else two consecutive row blocks of one head. CTAs (one per
-// SM) draw units from a counter, the longest of a sequence first; the kernel reads the sequences' starts on the
-// device, so one launch serves any mix of lengths. Roles of a CTA's 12 warps:
+// SM) draw units from a counter: sequences in their order, each one's last rows, which see the most keys, first (16 prompts
+// in ascending, descending and mixed order of length: 437 to 442 us). The kernel reads the sequences' starts on the
+// device, so one launch serves any mix of lengths. Few rows behind a long prefix leave SMs without a unit: 1 to 128 rows
+// behind 7994 keys take 110 us, whatever their number. Roles of a CTA's 12 warps:
 //   0     draws units, issues the TMA loads: Q tiles, then K and V tiles of 128 rows through a ring of four stages
 //   1     issues the MMAs: S_t = Q_t K^T and O_t += P_t V, S, P and O in tensor memory (S 128 columns a tile, P over
 //         the S it came from, O HD columns), V read as it lies (N-major operand)
@@ -33,9 +35,9 @@
 //
 // The tensor cores and the exponentials have as much to do: 2 x 128 x 128 exponentials and four 128 x 128 x HD products
 // take about 2048 cycles each at HD 128. A pair of tiles takes 3250: the MMA warp's waits and commits stand between the
-// products. 16,384 tokens of 64 / 8 heads in bf16 take 3.5 to 4.1 ms (the power limit's share varies), 1.07 to 1.26
-// PFLOP/s. Measured and not kept: an MMA warp for each query tile, whose products then interleave (17,495 tokens behind
-// prefixes, 28 / 4 heads: 414 -> 473 us), and two threads a row (469 us).
+// products. 16,384 tokens of 64 / 8 heads in bf16 take 4.18 ms, 1.05 PFLOP/s, at the power limit (SM clock 1.70 GHz).
+// Measured and not kept, each in turn with the kept kernel in single launches on 17,495 tokens behind prefixes, 28 / 4 heads:
+// an MMA warp for each query tile, whose products then interleave (14% slower), and two threads a row (13%).
 #include <mutex>
 
 #include "ops.cuh"

@@ -15,8 +15,8 @@
 // back and added in f32 by the threads that hold O in registers, while the tensor cores work on the next tile.
 //
 // Bound by the tensor cores for long prompts: 4 (f16) or 6 (bf16) products of 128 x 128 x HD a tile, of 512 cycles each
-// at HD 128 (20,545 tokens in prompts of up to 4096, 28 / 4 heads, f16: 880 us, 0.69 of their rate). By a unit's own
-// chain for short ones (2563 tokens in prompts of up to 512: 54 us).
+// at HD 128 (20,545 tokens in prompts of up to 4096, 28 / 4 heads: 886 us with f16 keys, 1187 with bf16, 0.69 and 0.77 of
+// their rate). By a unit's own chain for short ones (2563 tokens in prompts of up to 512: 53.5 us, 60.5 with bf16 keys).
 #include <mutex>
 
 #include "ops.cuh"

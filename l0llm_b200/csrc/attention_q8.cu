@@ -5,7 +5,7 @@
 // warps, one team per head, takes an equal run of that list, whatever the mix of lengths, which the kernel reads on
 // the device; one launch, one CTA per SM. So the teams that run side by side read the heads of the same slots, whole
 // cache rows, at the same time: with each head's list split on its own (hd bytes out of every row) the DRAM pages
-// were opened once per head, and 1.05 GB of 8 heads took 283 us where the same bytes of one head took 178. A run
+// were opened once per head, and 1.05 GB of 8 heads took 1.6 times as long as the same bytes of one head. A run
 // crosses items: the part of it inside one item is a segment. A warp takes every TEAM-th tile of its team's segment,
 // fetched by its own TMA two tiles ahead, segments ahead included, so HBM stays busy through their ends.
 //
@@ -25,8 +25,9 @@
 // several groups share has its parts joined, in group order, by the team that arrives last (a counter per first team,
 // which the joining team resets), so results do not depend on the order of arrival.
 //
-// Bound by HBM and instruction issue alike for long contexts (2 hd bytes a slot and KV head; 704 instructions a tile):
-// 514,036 slots of 8 heads of 128 in 221 us, 4.8 TB/s. By latency for short ones: 41,159 slots of 4 heads in 29 us.
+// Bound by latency between dependent instructions: at 142,126 slots of 8 heads of 128 half of the issue slots and half of
+// the DRAM rate are used, and 12 warps fill the registers. 514,036 slots take 218 us, 4.8 TB/s; 41,159 slots of 4 heads
+// 29.5 us, three tiles a warp.
 #include <mutex>
 
 #include "ops.cuh"
@@ -55,6 +56,8 @@ struct Q8Launch {
 // What a warp needs to know of one item, and the walk over items.
 // An item takes kItemUnits units and one for each of its tiles: starting and ending one costs as much as some twenty
 // tiles (query digits, the joining of states; 4 us of latency), and runs of equal length would be uneven without it.
+// With 0, 10, 20 and 40 units, 28 / 4 heads of 128, f32, in us: 16 sequences of up to 4096 slots 38, 31, 30, 28; 64 of up
+// to 1024 40, 32, 32, 33; 4 of up to 4096 25, 20, 19, 20; 64 of up to 16,384 169, 163, 159, 154.
 constexpr int kItemUnits = 20;
 
 struct Item {
@@ -245,7 +248,10 @@ __global__ void __launch_bounds__(warps_of(NT) * 32, 1) attn_q8_kernel(const __g
     const int U = pre[a.count];
     if (U == 0) return;
     // Long items: the CTA's warps share one run, which has the fewest parts to join. Short items (fewer tiles than
-    // two rounds of the CTA's warps): teams of four, so that more items are worked on at once.
+    // two rounds of the CTA's warps): teams of four, so that more items are worked on at once. All warps against four, 28 / 4
+    // heads of 128, f32, in us: one sequence of 32,768 slots 27 and 53; 4 of up to 4096 19 and 28; 16 of up to 4096 29 and
+    // 29; 64 of up to 512 29 and 24. The rule looks at tiles alone: many long items would gain 5% from four (64 of up to
+    // 16,384: 151 and 143), 4 of up to 512 lose 3 us to them (13 and 16).
     int items = 0;
     for (int w = 0; w < W; ++w) items += scan_s[w][1];
     const int team_warps = U >= static_cast<long long>(2 * W + kItemUnits) * items ? W : 4;

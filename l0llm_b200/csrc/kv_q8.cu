@@ -4,7 +4,7 @@
 // sequence that land in one block of slots; the row that opens it is its leader), for one KV head of K or V.
 // Every new value of a piece stays in registers between the two things done with it: the largest magnitude
 // (bits of |x| compared as integers, so an infinity or a NaN wins and the scale shows it) and the codes. So
-// the rows are read once and the codes written once. 22,200 bf16 rows of 8 heads of 128 take 38 us, 3.5 TB/s: a piece
+// the rows are read once and the codes written once. 22,167 bf16 rows of 8 heads of 128 take 35 us, 3.9 TB/s: a piece
 // is a chain of a fetch, a maximum over the CTA and a write, and two CTAs an SM (64 registers) hide some of it; three of
 // 40 registers spill and took 7% longer.
 //
@@ -198,8 +198,9 @@ __global__ void __launch_bounds__(512, 2) kv_q8_store_kernel(const KvQ8Params p,
 }
 
 // Load. A warp takes one packed row, K and V of it: 128 or 256 codes a step into 512 contiguous bytes. Bound by HBM:
-// 76,545 rows of 8 heads of 128 as f16 take 86 us, 5.5 TB/s. (Warps that took a run of rows, to find their sequence once,
-// took 87, and 194 instead of 156 for 4000 short sequences; finding one of 4096 takes three reads.)
+// 76,545 rows of 8 heads of 128 as f16 take 73 us, 6.4 TB/s; 86 before four steps' codes were loaded ahead of the first
+// step's stores. (Warps that took a run of rows, to find their sequence once, were no faster, and slower for 4000 short
+// sequences, 194 against 156 us; finding one of 4096 takes three reads.)
 template <typename T>
 __global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p) {
     constexpr int VEC = 16 / sizeof(T);  // codes of a thread's step: 16 bytes out
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(256) kv_q8_load_kernel(const KvQ8Params p) {
                     v[4 * j + 2] = b.x * scale[k];
                     v[4 * j + 3] = b.y * scale[k];
                 }
-                // f32 rows go past the L2: 22,167 rows stored and read back took 78.5 us, now 70.7. 16-bit ones would lose 1%.
+                // f32 rows go past the L2: 22,167 rows stored and read back 78.5 -> 70.7 us. 16-bit ones would lose 1%.
                 if constexpr (VEC == 4) __stcs(reinterpret_cast<float4*>(dst + c), make_float4(v[0], v[1], v[2], v[3]));
                 else store8(dst + c, v);
             }
